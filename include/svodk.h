@@ -36,7 +36,10 @@ typedef enum svodk_dtype {
   SVODK_F32 = 2,
   SVODK_I32 = 3,
   SVODK_I64 = 4,
-  SVODK_BOOL = 5 /* one byte per element, nonzero = true */
+  SVODK_BOOL = 5, /* one byte per element, nonzero = true */
+  /* A cache in pages only (svodk_pages): */
+  SVODK_E4M3 = 6, /* 8-bit floats of four exponent and three significand bits, no infinities (OCP e4m3fn) */
+  SVODK_E8M0 = 7  /* a power of two, 2^(byte - 127) */
 } svodk_dtype;
 
 /*
@@ -222,6 +225,70 @@ int svodk_attention_packed(const svodk_tensor *qkv, int32_t heads, int32_t kv_he
  * B <= 8192.  One small launch on the stream.
  */
 int svodk_order_rows(const svodk_tensor *keys, const svodk_tensor *order, void *hip_stream);
+
+/*
+ * A key/value cache in pages.  It has no counterpart in the reference, whose caches are whole rows
+ * (svodk_cache): sequences of any length share one pool, in pages of `page` tokens that need not lie in order.
+ *
+ * Sequence b has lens[b] tokens in the cache.  The last starts[b+1] - starts[b] of them are the call's new
+ * ones and lie in rows starts[b] .. starts[b+1]-1 of its packed operands [N, heads, D], one sequence after
+ * the other (none, one or thousands each): its i-th new token stands at position
+ * lens[b] - (starts[b+1] - starts[b]) + i.  The token at position p is row p % page of page table[b, p / page]
+ * of the pools, which hold a KV head's rows of a page side by side.  Rows of the packed operands outside every
+ * sequence are neither read nor written.
+ *
+ * Pools are of 16 bits (the operands' type) or of 8: then a row of D codes has a scale, a power of two, and
+ * stands for code * scale.  Row x is stored with the scale 2^e, e the least whole number from -117 on with
+ * max|x| <= 448 * 2^e over its finite values, and codes x / 2^e rounded to the nearest even; codes that would
+ * stand for more than the operands' type holds end at 240 * 2^e.  An infinity or a NaN is stored as NaN.
+ *
+ * `page` is a power of two from 16 to 1024, D 64, 128 or 256; others answer SVODK_GRAPH_SHAPE.  The table's
+ * entries, lengths and starts are device data that no host check reads: they are held inside the pool, the
+ * table (lens[b] <= columns * page) and the packed operands, so that a bad one gives a wrong result and never
+ * an access out of bounds.  A sequence with fewer tokens than new rows has no position for the first of them:
+ * they are not stored and see no key.  Rows in two sequences at once (starts that descend) may be left out.
+ */
+typedef struct svodk_pages {
+  const svodk_tensor *k, *v;             /* [pages, kv_heads, page, D], one type */
+  const svodk_tensor *k_scale, *v_scale; /* [pages, kv_heads, page] SVODK_E8M0 with pools of SVODK_E4M3, else NULL */
+  const svodk_tensor *table;             /* [B, columns] I32; entries past a sequence's pages are not used */
+  const svodk_tensor *lens;              /* [B] I32 or I64 */
+  const svodk_tensor *starts;            /* [B + 1] I32 or I64, ascending */
+} svodk_pages;
+
+/*
+ * The new tokens' keys and values k and v [N, kv_heads, D] into their pages.  Each call in flight must have its
+ * pages to itself, and of a page that the tokens of two sequences are written to in one call, at the same rows,
+ * either's remain (with 8 bits, one's codes perhaps under the other's scale).
+ */
+int svodk_write_pages(const svodk_tensor *k, const svodk_tensor *v, const svodk_pages *pages, void *hip_stream);
+
+/*
+ * And back: positions 0 .. T-1 of each sequence into k and v [B, T, kv_heads, D], the layout of svodk_attention's
+ * keys, zeros from its end on.  The outputs are of the pools' type, or of either 16-bit type where those hold 8
+ * bits.  `starts` may be NULL.
+ */
+int svodk_read_pages(const svodk_pages *pages, const svodk_tensor *k, const svodk_tensor *v, void *hip_stream);
+
+/*
+ * Attention of the new tokens' queries q [N, heads, D] over their sequences' pages, into out [N, heads, D]: the
+ * op of svodk_attention with each query at its token's position p.  causal: keys 0 .. p, the token's own among
+ * them (svodk_write_pages comes first); a window: keys p - left .. p + right; neither: all lens[b].  A query that
+ * sees no key comes out as zeros.  Of the options causal, window, scale, splits and workspace count; any other
+ * that is set answers SVODK_GRAPH_CONFIG, as does a named count of splits without the workspace it needs.
+ * More than 128 query heads a KV head answer SVODK_GRAPH_SHAPE.
+ *
+ * `splits` = 0 splits the keys of long sequences where the workspace svodk_attention_paged_workspace asks for
+ * is lent, by all the sequences' lengths, which the device looks at: a row's last bits may depend on the other
+ * sequences'.  1 keeps the keys whole, n > 1 gives every tile of rows n splits, or as many as it has key blocks of
+ * 64.  What the workspace holds at first does not matter; no two launches in flight may have the same.
+ * Values of keys that a row does not see are multiplied by zero where other rows of its tile see them: they
+ * have to be finite (svodk_attention does the same).  Rows past a sequence's end in its last page are not read.
+ */
+int svodk_attention_paged(const svodk_tensor *q, const svodk_pages *pages, const svodk_attn *opts, const svodk_tensor *out,
+                          void *hip_stream);
+/* Bytes of `workspace` that svodk_attention_paged wants for these operands; 0 where it never splits.  Pure, no device. */
+int64_t svodk_attention_paged_workspace(const svodk_tensor *q, const svodk_pages *pages, const svodk_attn *opts);
 
 /*
  * Bytes of `workspace` svodk_attention needs for these operands and options:

@@ -17,12 +17,15 @@ from .ops import (  # noqa: F401
     Linear,
     Rotary,
     OpError,
+    Pages,
     Qkv,
     add_layer_norm,
     add_rms_norm,
     attention,
     attention_noalloc,
     attention_packed,
+    attention_paged,
+    attention_paged_workspace,
     noalloc_scratch_bytes,
     DECODE_ROWS_DEFAULT,
     tune_decode,
@@ -39,6 +42,8 @@ from .ops import (  # noqa: F401
     plan_attention,
     plan_heads,
     plan_norm,
+    read_pages,
     rms_norm,
     supported,
+    write_pages,
 )

@@ -16,8 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsvodk_gfx950.so")
 HOST = os.path.join(HERE, "_host.so")  # the Python side's calls (csrc/host.cpp), a module of this package
-SOURCES = ["ops.cpp", "heads_kernel.hip", "attention_kernel.hip", "combine_kernel.hip", "rows_kernel.hip",
-           "linear_kernel.hip", "linear_few_kernel.hip", "decode_kernel.hip"]
+SOURCES = ["ops.cpp", "pages.cpp", "heads_kernel.hip", "attention_kernel.hip", "combine_kernel.hip", "rows_kernel.hip",
+           "linear_kernel.hip", "linear_few_kernel.hip", "decode_kernel.hip", "pages_kernel.hip", "paged_kernel.hip"]
 
 # Packed-FP32 VALU ops are switched off for device code; the host pass of hipcc
 # does not know the feature and says so, which is harmless.
@@ -31,7 +31,8 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang"
 # The last one keeps an atomic add what the source says (one lane, no wait on the spot): the
 # rewrite for wave-uniform operands waits for the answer where the add is issued.
 EXTRA_FLAGS = {"attention_kernel.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-kernarg-preload-count=16",
-                                        "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
+                                        "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
+               "paged_kernel.hip": ["-fno-honor-nans"]}  # the same steps
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-command-line-argument"]
 
 
@@ -42,9 +43,9 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (looked at $HIPCC, PATH and /opt/rocm/bin)")
 
 
-# The attention source is compiled once per head size and once for what does not depend on it
+# An attention source is compiled once per head size and once for what does not depend on it
 # (its SVODK_HEAD macro), side by side: one translation unit of every instantiation takes minutes.
-ATTENTION_PARTS = [0, 32, 48, 64, 128, 256]
+PARTS = {"attention_kernel.hip": [0, 32, 48, 64, 128, 256], "paged_kernel.hip": [0, 64, 128, 256]}
 
 
 def build(verbose: bool = False) -> str:
@@ -57,7 +58,7 @@ def build(verbose: bool = False) -> str:
     jobs = []
     for src in SOURCES:
         stem = os.path.splitext(src)[0]
-        parts = [(f"_h{h}", [f"-DSVODK_HEAD={h}"]) for h in ATTENTION_PARTS] if src == "attention_kernel.hip" else [("", [])]
+        parts = [(f"_h{h}", [f"-DSVODK_HEAD={h}"]) for h in PARTS[src]] if src in PARTS else [("", [])]
         for suffix, defines in parts:
             obj = os.path.join(objdir, stem + suffix + ".o")
             jobs.append((obj, [cc, "-x", "hip", *DEVICE_FLAGS, *COMMON_FLAGS, *EXTRA_FLAGS.get(src, []), *defines,

@@ -156,6 +156,12 @@ constexpr unsigned kStream = 1;  // a workgroup walks several query tiles
 constexpr unsigned kRanged = 2;  // per-row key ranges: window, chunk mask, segment starts
 constexpr unsigned kBiased = 4;  // an additive bias joins the scaled scores
 constexpr unsigned kSided = 8;   // one of a tile's two sides: every other key block is this wave's
+constexpr unsigned kPaged = 16;  // the keys lie in pages
+constexpr unsigned kCoded = 32;  // and are e4m3 codes there, widened on their way into LDS
+
+// What a wave knows of its keys' pages: nothing where they lie in rows.
+template <int D, int NW, bool PAGED, bool CODED>
+struct Pages {};
 
 // Everything a wave carries through the key loop.
 template <int D, int NW, bool F16, unsigned FLAGS>
@@ -194,7 +200,7 @@ struct Wave {
   int lo_first, lo_last, hi_first, hi_last;
   // per-lane addressing
   // global byte offsets of this lane's chunk in this wave's fills of a tile (one per swizzle phase)
-  static constexpr int NS = Tile<D>::sources(NW);
+  static constexpr int NS = (FLAGS & kPaged) ? 1 : Tile<D>::sources(NW);
   int k_src[NS], v_src[NS];
   int k_read[KS], v_read[DB];
   // state
@@ -213,7 +219,17 @@ struct Wave {
   const uint8_t *nxt_k, *nxt_v;
   int64_t nxt_bytes;
   int nxt_end, end_even;
+  // Keys in pages (paged_kernel.hip's fills).
+  Pages<D, NW, (FLAGS & kPaged) != 0, (FLAGS & kCoded) != 0> pages;
 };
+
+// A tile's fills where its keys lie in pages: defined beside Pages.
+template <int D, int NW, bool F16, unsigned FLAGS>
+__device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot);
+template <int D, int NW, bool F16, unsigned FLAGS>
+__device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot);
+template <int D, int NW, bool F16, unsigned FLAGS>
+__device__ __forceinline__ void land_pages(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk, int par);
 
 // The fills are issued as raw instructions: the compiler's wait-count pass treats an LDS fill
 // it knows about as aliasing every later LDS read and would park the wave on the NEXT tile's
@@ -242,20 +258,28 @@ __device__ __forceinline__ void fill_tile(const Wave<D, NW, F16, FLAGS> &w, cons
 // Block `n` of the stream of blocks that starts with this item's: the item's own while n < end,
 // then (past the padding to an even count) the next item's.  Nothing past either.
 template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void fill_k(const Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
-  const int at = w.lds0 + slot * Tile<D>::kBytes;
-  if (n < w.end)
-    fill_tile<D, NW>(w, w.k_base, w.kv_bytes, n, at, w.k_src, w.kv_row_bytes);
-  else if ((FLAGS & kStream) && n >= w.end_even && n - w.end_even < w.nxt_end)
-    fill_tile<D, NW>(w, w.nxt_k, w.nxt_bytes, n - w.end_even, at, w.k_src, w.kv_row_bytes);
+__device__ __forceinline__ void fill_k(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
+  if constexpr ((FLAGS & kPaged) != 0) {
+    fill_k_pages<D, NW>(w, n, slot);
+  } else {
+    const int at = w.lds0 + slot * Tile<D>::kBytes;
+    if (n < w.end)
+      fill_tile<D, NW>(w, w.k_base, w.kv_bytes, n, at, w.k_src, w.kv_row_bytes);
+    else if ((FLAGS & kStream) && n >= w.end_even && n - w.end_even < w.nxt_end)
+      fill_tile<D, NW>(w, w.nxt_k, w.nxt_bytes, n - w.end_even, at, w.k_src, w.kv_row_bytes);
+  }
 }
 template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void fill_v(const Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
-  const int at = w.lds0 + (2 + slot) * Tile<D>::kBytes;
-  if (n < w.end)
-    fill_tile<D, NW>(w, w.v_base, w.kv_bytes, n, at, w.v_src, w.kv_row_bytes);
-  else if ((FLAGS & kStream) && n >= w.end_even && n - w.end_even < w.nxt_end)
-    fill_tile<D, NW>(w, w.nxt_v, w.nxt_bytes, n - w.end_even, at, w.v_src, w.kv_row_bytes);
+__device__ __forceinline__ void fill_v(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
+  if constexpr ((FLAGS & kPaged) != 0) {
+    fill_v_pages<D, NW>(w, n, slot);
+  } else {
+    const int at = w.lds0 + (2 + slot) * Tile<D>::kBytes;
+    if (n < w.end)
+      fill_tile<D, NW>(w, w.v_base, w.kv_bytes, n, at, w.v_src, w.kv_row_bytes);
+    else if ((FLAGS & kStream) && n >= w.end_even && n - w.end_even < w.nxt_end)
+      fill_tile<D, NW>(w, w.nxt_v, w.nxt_bytes, n - w.end_even, at, w.v_src, w.kv_row_bytes);
+  }
 }
 
 // A key mask row is read 64 keys (one per lane) a block, one block ahead: the load is issued
@@ -608,6 +632,7 @@ __device__ __forceinline__ void hot_step(Wave<D, NW, F16, FLAGS> &w, const uint8
     bm = __builtin_fmaxf(p.a, p.b);
   }
   w.l_run = w.l_run * corr + ((bs[0] + bs[1]) + (bs[2] + bs[3]));
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, PAR);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
   __syncthreads();
 }
@@ -664,16 +689,18 @@ __device__ __forceinline__ void edge_step(Wave<D, NW, F16, FLAGS> &w, const uint
       bm = row_max(sv);
     }
   }
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, par);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
   __syncthreads();
 }
 
 // A step of a wave with nothing to compute: fills and the barrier only.
 template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void idle_step(Wave<D, NW, F16, FLAGS> &w, int blk) {
+__device__ __forceinline__ void idle_step(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk) {
   const int par = blk & 1;
   fill_v<D, NW>(w, blk + 1, par ^ 1);
   fill_k<D, NW>(w, blk + 2, par);
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, smem, blk, par);
   __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 }

@@ -14,6 +14,7 @@
 #include <ATen/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -38,6 +39,13 @@ struct Abi {
   decltype(&svodk_order_rows) order_rows;
 };
 Abi abi;
+struct PagesAbi {
+  decltype(&svodk_write_pages) write_pages;
+  decltype(&svodk_read_pages) read_pages;
+  decltype(&svodk_attention_paged) attention_paged;
+  decltype(&svodk_attention_paged_workspace) attention_paged_workspace;
+};
+PagesAbi pages_abi;
 PyObject *op_error;  // ops.OpError
 PyObject *finish;    // ops._finish(op, status): raises what a status other than 0 stands for
 PyObject *dtypes[6];  // torch's dtype objects, by svodk_dtype (for ops._fresh)
@@ -89,7 +97,8 @@ struct Kept {
 #define SVODK_NAMES(X)                                                                                              \
   X(causal) X(keys) X(kind) X(tensor) X(window) X(chunk) X(seg_start) X(cache) X(head_start) X(kv_heads) X(row_map) \
   X(appended) X(app_lens) X(bias) X(splits) X(scale) X(batch_live) X(row_order) X(heads) X(head_dim) X(q_norm)      \
-  X(k_norm) X(eps) X(rope) X(cos) X(sin) X(act) X(gated) X(residual) X(into)
+  X(k_norm) X(eps) X(rope) X(cos) X(sin) X(act) X(gated) X(residual) X(into) X(k) X(v) X(table) X(lens) X(starts)    \
+  X(scales)
 struct Names {
 #define SVODK_NAME(n) PyObject *n;
   SVODK_NAMES(SVODK_NAME)
@@ -142,9 +151,14 @@ int dtype_of(at::ScalarType t) {
   }
 }
 
-void describe(PyObject *o, svodk_tensor &d) {
+// A pool of pages or its scales: the 8-bit types are theirs alone.
+int pool_dtype_of(at::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? SVODK_E4M3 : t == at::kFloat8_e8m0fnu ? SVODK_E8M0 : dtype_of(t);
+}
+
+void describe(PyObject *o, svodk_tensor &d, int (*type_of)(at::ScalarType) = dtype_of) {
   const at::Tensor &t = tensor(o);
-  d.dtype = dtype_of(t.scalar_type());
+  d.dtype = type_of(t.scalar_type());
   if (d.dtype < 0) {
     Ref dt(PyObject_GetAttrString(o, "dtype"));
     Ref text(PyUnicode_FromFormat("unsupported element type %S", (PyObject *)dt));
@@ -587,19 +601,143 @@ PyObject *py_order_rows(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   SVODK_END
 }
 
+// A Pages' fields as the ABI's struct, with the descriptors that it points to.
+struct PagesCall {
+  svodk_pages p{};
+  svodk_tensor k, v, k_scale, v_scale, table, lens, starts;
+  Kept kept;
+  PyObject *pool;  // the key pool: kept
+
+  explicit PagesCall(PyObject *pages) {
+    pool = kept(get(pages, names.k));
+    describe(pool, k, pool_dtype_of), describe(kept(get(pages, names.v)), v, pool_dtype_of);
+    p.k = &k, p.v = &v;
+    describe(kept(get(pages, names.table)), table), describe(kept(get(pages, names.lens)), lens);
+    p.table = &table, p.lens = &lens;
+    p.starts = maybe_attr(kept, pages, names.starts, starts);
+    Ref scales(get(pages, names.scales));
+    if (scales != Py_None) {
+      describe(kept(PySequence_GetItem(scales, 0)), k_scale, pool_dtype_of);
+      describe(kept(PySequence_GetItem(scales, 1)), v_scale, pool_dtype_of);
+      p.k_scale = &k_scale, p.v_scale = &v_scale;
+    }
+  }
+};
+
+// (k, v, pages)
+PyObject *py_write_pages(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  SVODK_ARGS(3, "write_pages")
+  SVODK_BEGIN
+  PagesCall call(args[2]);
+  svodk_tensor kd, vd;
+  describe(args[0], kd), describe(args[1], vd);
+  void *stream = stream_of(tensor(args[0]));
+  const int status = unlocked(tensor(args[0]), [&] { return pages_abi.write_pages(&kd, &vd, &call.p, stream); });
+  Ref none(held(Py_None));
+  return answer("write_pages", status, none);
+  SVODK_END
+}
+
+// (pages, tokens, dtype, out, fresh); out and the answer: (k, v)
+PyObject *py_read_pages(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  SVODK_ARGS(5, "read_pages")
+  SVODK_BEGIN
+  PagesCall call(args[0]);
+  const int64_t tokens = as_int(args[1]);
+  PyObject *made = args[3];
+  if (made != Py_None) {
+    made = held(made);
+  } else {
+    if (tokens < 0) op_failed("Shape", "read_pages: a negative count of tokens");
+    at::ScalarType type = tensor(call.pool).scalar_type();
+    if (args[2] != Py_None) {
+      if (!THPDtype_Check(args[2])) {
+        PyErr_SetString(PyExc_TypeError, "read_pages: dtype is a torch.dtype or None");
+        throw Raised();
+      }
+      type = reinterpret_cast<THPDtype *>(args[2])->scalar_type;
+    } else if (type == at::kFloat8_e4m3fn) {
+      type = at::kBFloat16;
+    }
+    if (dtype_of(type) < 0) op_failed("Dtype", "read_pages: the rows are of a 16-bit type");
+    // With descriptors the op will not take: let it word the error; the outputs are never touched.
+    const bool fits = call.k.rank == 4 && call.table.rank == 2;
+    const int64_t b = fits ? call.table.shape[0] : 0, h = fits ? call.k.shape[1] : 0, d = fits ? call.k.shape[3] : 0;
+    Ref k(allocate(args[4], {b, tokens, h, d}, type, call.pool)), v(allocate(args[4], {b, tokens, h, d}, type, call.pool));
+    made = PyTuple_Pack(2, (PyObject *)k, (PyObject *)v);
+  }
+  Ref out(made);
+  svodk_tensor kd, vd;
+  Kept kept;
+  describe(kept(PySequence_GetItem(out, 0)), kd), describe(kept(PySequence_GetItem(out, 1)), vd);
+  void *stream = stream_of(tensor(call.pool));
+  const int status = unlocked(tensor(call.pool), [&] { return pages_abi.read_pages(&call.p, &kd, &vd, stream); });
+  return answer("read_pages", status, out);
+  SVODK_END
+}
+
+// (q, pages, opts, out, workspace, fresh)
+PyObject *py_attention_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  SVODK_ARGS(6, "attention_paged")
+  SVODK_BEGIN
+  PyObject *q = args[0], *fresh = args[5];
+  Ref out(args[3] == Py_None ? allocate_like(fresh, q) : held(args[3]));
+  PagesCall pages(args[1]);
+  AttnCall call(args[2]);
+  svodk_tensor qd, od;
+  describe(q, qd), describe(out, od);
+  Ref lent(held(args[4]));
+  if (lent == Py_None && call.a.splits != 1) {
+    const int64_t need = pages_abi.attention_paged_workspace(&qd, &pages.p, &call.a);
+    if (need > 0) lent.take(allocate(fresh, {need}, at::kByte, q));
+  }
+  if (lent != Py_None) {
+    const at::Tensor &t = tensor(lent);
+    call.a.workspace = t.data_ptr(), call.a.workspace_bytes = (int64_t)t.numel() * (int64_t)t.element_size();
+  }
+  void *stream = stream_of(tensor(q));
+  const int status = unlocked(tensor(q), [&] { return pages_abi.attention_paged(&qd, &pages.p, &call.a, &od, stream); });
+  return answer("attention_paged", status, out);
+  SVODK_END
+}
+
+// (q, pages, opts): the bytes of workspace that the call wants (svodk_attention_paged_workspace)
+PyObject *py_attention_paged_workspace(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  SVODK_ARGS(3, "attention_paged_workspace")
+  SVODK_BEGIN
+  PagesCall pages(args[1]);
+  AttnCall call(args[2]);
+  svodk_tensor qd;
+  describe(args[0], qd);
+  return PyLong_FromLongLong(pages_abi.attention_paged_workspace(&qd, &pages.p, &call.a));
+  SVODK_END
+}
+
+// A function's address out of {function name: address}.
+void *address(PyObject *table, const char *name) {
+  PyObject *x = PyDict_GetItemString(table, name);
+  void *p = x == nullptr ? nullptr : PyLong_AsVoidPtr(x);
+  if (p == nullptr && !PyErr_Occurred()) PyErr_Format(PyExc_KeyError, "%s", name);
+  return p;
+}
+#define SVODK_TAKE(f) \
+  if ((found.f = (decltype(found.f))address(table, "svodk_" #f)) == nullptr) return nullptr;
+
+// ({function name: address}): the functions of a cache in pages
+PyObject *py_bind_pages(PyObject *, PyObject *args) {
+  PyObject *table;
+  if (!PyArg_ParseTuple(args, "O!", &PyDict_Type, &table)) return nullptr;
+  PagesAbi found;
+  SVODK_TAKE(write_pages) SVODK_TAKE(read_pages) SVODK_TAKE(attention_paged) SVODK_TAKE(attention_paged_workspace)
+  pages_abi = found;
+  Py_RETURN_NONE;
+}
+
 // ({function name: address}, OpError, _finish, (dtype by svodk_dtype, ...))
 PyObject *py_bind(PyObject *, PyObject *args) {
   PyObject *table, *error, *done, *types;
   if (!PyArg_ParseTuple(args, "O!OOO!", &PyDict_Type, &table, &error, &done, &PyTuple_Type, &types)) return nullptr;
-  auto address = [&](const char *name) -> void * {
-    PyObject *x = PyDict_GetItemString(table, name);
-    void *p = x == nullptr ? nullptr : PyLong_AsVoidPtr(x);
-    if (p == nullptr && !PyErr_Occurred()) PyErr_Format(PyExc_KeyError, "%s", name);
-    return p;
-  };
   Abi found;
-#define SVODK_TAKE(f) \
-  if ((found.f = (decltype(found.f))address("svodk_" #f)) == nullptr) return nullptr;
   SVODK_TAKE(attention) SVODK_TAKE(attention_noalloc) SVODK_TAKE(attention_packed) SVODK_TAKE(attention_workspace)
   SVODK_TAKE(heads) SVODK_TAKE(linear) SVODK_TAKE(layer_norm) SVODK_TAKE(add_layer_norm) SVODK_TAKE(rms_norm)
   SVODK_TAKE(add_rms_norm) SVODK_TAKE(order_rows)
@@ -621,6 +759,7 @@ PyObject *py_bind(PyObject *, PyObject *args) {
 #define SVODK_FAST(name, fn) {name, (PyCFunction)(void (*)(void))(fn), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, nullptr},
+    {"bind_pages", py_bind_pages, METH_VARARGS, nullptr},
     SVODK_FAST("attention", py_attention),
     SVODK_FAST("attention_noalloc", py_attention_noalloc),
     SVODK_FAST("attention_workspace", py_attention_workspace),
@@ -630,6 +769,10 @@ PyMethodDef methods[] = {
     SVODK_FAST("layer_norm", py_norm<true>),
     SVODK_FAST("rms_norm", py_norm<false>),
     SVODK_FAST("order_rows", py_order_rows),
+    SVODK_FAST("write_pages", py_write_pages),
+    SVODK_FAST("read_pages", py_read_pages),
+    SVODK_FAST("attention_paged", py_attention_paged),
+    SVODK_FAST("attention_paged_workspace", py_attention_paged_workspace),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

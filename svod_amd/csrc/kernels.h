@@ -200,6 +200,53 @@ constexpr int heads_together(int d, uint32_t heads_splits, uint32_t kv_heads) {
 constexpr int kMostMergedSplits = 64;
 constexpr int kArrivalBytes = 128;
 inline int64_t decode_arrival_bytes(const AttnArgs &a) { return (int64_t)a.batch * a.kv_heads * kArrivalBytes; }
+// A key/value cache in pages (svodk_pages): pools [pages, kv_heads, 1 << page_log2, d], the sequences' tables, lengths and packed
+// rows.  No counterpart in the reference, whose caches are rows (tk/src/ops/attention.rs:39-56).
+struct PagesArgs {
+  void *k, *v;              // 16-bit values, or e4m3 codes with their rows' scales
+  void *k_scale, *v_scale;  // [pages, kv_heads, page] bytes e + 127, null where the pools hold 16 bits
+  const int32_t *table;     // [batch, columns]
+  const void *lens;         // [batch] i32 or i64
+  const void *starts;       // [batch + 1] i32 or i64
+  int32_t batch, columns, pages, kv_heads, d, page_log2;
+  int32_t rows;             // of the packed operands
+  int32_t lens_i64, starts_i64;
+  int32_t f16;              // the 16-bit operands are f16, not bf16
+};
+// k and v [rows, kv_heads, d] into the pages.
+hipError_t launch_write_pages(const PagesArgs &a, const void *k, const void *v, hipStream_t stream);
+// The first `tokens` positions of each sequence out of them into k and v [batch, tokens, kv_heads, d], zeros past its end.
+hipError_t launch_read_pages(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream);
+// Head sizes the kernels of pages are built for, and page sizes.
+bool pages_support(int64_t d);
+constexpr int32_t kLeastPage = 16, kMostPage = 1024;
+
+// Attention of the packed rows over their sequences' pages.
+struct PagedArgs {
+  PagesArgs pages;
+  const void *q;  // [rows, heads, d]
+  void *o;
+  int32_t heads;
+  int32_t causal;
+  int32_t win_left, win_right;  // as in AttnArgs; win_left < 0 = no window
+  float scale;
+  int32_t splits;    // key splits a tile: 0 = the device's choice, 1 = none, or as many as named where there are the blocks
+  float *workspace;  // paged_slots(a) * paged_slot_floats(a) floats; null with `splits` 1
+};
+// The most query heads a KV head serves: a tile holds whole tokens.
+constexpr int32_t kMostPagedGroup = 128;
+// A call's form: query rows of a tile, 32 or 128.
+int paged_tile_rows(const PagedArgs &a);
+// The most partial states a call can leave, and the size of one.
+int64_t paged_slots(const PagedArgs &a);
+int64_t paged_slot_floats(const PagedArgs &a);
+int64_t paged_workgroups(const PagedArgs &a);
+hipError_t launch_paged(const PagedArgs &a, hipStream_t stream);
+const char *paged_config(const PagedArgs &a);
+// One head size's kernels each.
+hipError_t launch_paged_d64(const PagedArgs &a, hipStream_t stream);
+hipError_t launch_paged_d128(const PagedArgs &a, hipStream_t stream);
+hipError_t launch_paged_d256(const PagedArgs &a, hipStream_t stream);
 // One head size's kernels each (launch_attention picks by AttnArgs::d).
 hipError_t launch_attention_d32(const AttnArgs &a, hipStream_t stream);
 hipError_t launch_attention_d48(const AttnArgs &a, hipStream_t stream);

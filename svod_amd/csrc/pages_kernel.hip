@@ -1,0 +1,220 @@
+// A key/value cache in pages, for gfx950 (MI355X): new tokens' keys and values into it, and its sequences out of it.
+//
+// Written as they are, or in 8 bits.  A row of 8 bits is e4m3 codes c_i and one exponent e, the row's values 2^e c_i:
+//   e = the least whole number with max |x| <= 448 * 2^e (448 is e4m3's largest), from -117 on;   c_i = x_i * 2^-e to the nearest even
+// over the row's finite values.  A power of two, not max / 448: x * 2^-e is exact, so that a value is rounded once and alike wherever
+// it is computed, and a code times 2^e is exact in bf16 and, for rows that came from f16, in f16.  e4m3 gives up nothing for it but its range's last
+// bit.  Where 256 * 2^e lies past the type's largest value (f16: rows that reach past 57344, e = 8), codes end at 240: a value in
+// 63488 .. 65504 is within 2^-4 of 61440 still, and no finite value comes back infinite.  An infinity or a NaN comes back as NaN.
+//
+// Both directions are copies, bound by memory.  A wave's 1 KiB of 16-bit rows are neighbouring positions of one KV head: the pool's side is
+// a run without gaps (a page holds a head's rows side by side), the other's are whole rows of D values.
+#include <hip/hip_runtime.h>
+
+#include "convert.h"
+#include "kernels.h"
+#include "launch.h"
+#include "pages.h"
+
+namespace svodk {
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+constexpr int kWaves = 4;
+
+// The maximum of a value of [0, 2^31) over the LANES lanes of a row (neighbours, 8 to 32 of them).
+template <int LANES>
+__device__ __forceinline__ int row_most(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true));   // quad_perm: 1, 0, 3, 2
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true));   // quad_perm: 2, 3, 0, 1
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true));  // row_half_mirror
+  if constexpr (LANES >= 16) x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true));  // row_mirror
+  if constexpr (LANES >= 32) x = max(x, __shfl_xor(x, 16));
+#endif
+  return x;
+}
+
+// Eight values of a row of LANES lanes as codes; `e` the row's exponent.
+template <bool F16, int LANES>
+__device__ __forceinline__ u32x2 to_codes(const u32x4 &w, int &e) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+  constexpr int kTop = F16 ? 8 : 120;  // with it a code of 256 is past the type's largest value
+  int most = 0;  // the largest finite magnitude's bits
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
+    most = max(most, (int)(lo < kInf ? lo : 0u));
+    most = max(most, (int)(hi < kInf ? hi : 0u));
+  }
+  most = row_most<LANES>(most);
+  uint32_t bits;  // as an f32's
+  if constexpr (F16)
+    bits = __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)most));
+  else
+    bits = (uint32_t)most << 16;
+  // 448 = 1.75 * 2^8: one more where the significand is past 1.75.
+  e = max((int)((bits + 0x1fffffu) >> 23) - 135, -117);
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  const float limit = e >= kTop ? 240.0f : 448.0f;
+  float x[8];
+  widen<F16>(w, x);
+  uint32_t out[2];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    // A value that is not finite is left out of the clamp and made NaN: e4m3 has no infinity.
+    const uint32_t half = (i & 1) ? (w[i / 2] >> 16) & 0x7fffu : w[i / 2] & 0x7fffu;
+    const float y = __builtin_fminf(__builtin_fmaxf(x[i] * down, -limit), limit);
+    x[i] = half < kInf ? y : __uint_as_float(0x7fc00000u);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    int word = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+    word = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], word, true);
+    out[i] = (uint32_t)word;
+  }
+  return u32x2{out[0], out[1]};
+#else
+  return u32x2{};
+#endif
+}
+
+// ---- into the pages.  A wave takes 64 / LANES packed rows of one KV head, keys and values.
+template <int D, bool F16, bool CODED>
+__global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes;
+  const int lane = (int)__builtin_amdgcn_workitem_id_x() & 63;
+  const uint32_t wave = __builtin_amdgcn_workgroup_id_x() * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_amdgcn_workitem_id_x() >> 6);
+  const uint32_t group = wave / (uint32_t)p.kv_heads;
+  const int head = (int)(wave - group * (uint32_t)p.kv_heads);
+  const int64_t row0 = (int64_t)group * kRows;
+  if (row0 >= p.rows) return;
+  const int64_t row = row0 + lane / kLanes;
+  const bool there = row < p.rows;
+  const int64_t from = ((there ? row : row0) * p.kv_heads + head) * D + lane % kLanes * 8;
+  const u32x4 xk = *reinterpret_cast<const u32x4 *>(k + from), xv = *reinterpret_cast<const u32x4 *>(v + from);
+  // The sequence and the position of each of the wave's rows: the sequences a lane each, 64 at a time.
+  int b = -1, at = -1;
+  for (int base = 0; base < p.batch; base += 64) {
+    Sequence s{};
+    if (base + lane < p.batch) s = sequence_at(p, base + lane);
+    int found = 0;
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      const int64_t in = row0 + r - s.start;
+      const uint64_t here = __builtin_amdgcn_ballot_w64(in >= 0 && in < s.fresh);
+      if (here != 0) {
+        found++;
+        const int one = __builtin_ctzll(here);
+        const int position = __builtin_amdgcn_readlane(s.base() - s.start, one) + (int)(row0 + r);
+        if (lane / kLanes == r && b < 0) b = base + one, at = position;
+      }
+    }
+    if (found == kRows) break;
+  }
+  if (!there || b < 0 || at < 0) return;  // a row of no sequence, or past what the length has room for
+  const int64_t to = page_row(p, page_at(p, b, at >> p.page_log2), head) + (at & ((1 << p.page_log2) - 1));
+  if constexpr (CODED) {
+    int ek, ev;
+    const u32x2 ck = to_codes<F16, kLanes>(xk, ek), cv = to_codes<F16, kLanes>(xv, ev);
+    *reinterpret_cast<u32x2 *>((uint8_t *)p.k + to * D + lane % kLanes * 8) = ck;
+    *reinterpret_cast<u32x2 *>((uint8_t *)p.v + to * D + lane % kLanes * 8) = cv;
+    if (lane % kLanes == 0) {
+      ((uint8_t *)p.k_scale)[to] = (uint8_t)(ek + 127);
+      ((uint8_t *)p.v_scale)[to] = (uint8_t)(ev + 127);
+    }
+  } else {
+    *reinterpret_cast<u32x4 *>((uint16_t *)p.k + to * D + lane % kLanes * 8) = xk;
+    *reinterpret_cast<u32x4 *>((uint16_t *)p.v + to * D + lane % kLanes * 8) = xv;
+  }
+#endif
+}
+
+// ---- and out of them.  A wave takes 64 / LANES neighbouring positions of one (sequence, KV head): no page ends inside.
+template <int D, bool F16, bool CODED>
+__global__ __launch_bounds__(kWaves * 64) void read_pages_kernel(PagesArgs p, int tokens, uint32_t groups, uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes;
+  static_assert(kRows <= kLeastPage, "a wave's rows lie in one page");
+  const int lane = (int)__builtin_amdgcn_workitem_id_x() & 63;
+  const uint32_t wave = __builtin_amdgcn_workgroup_id_x() * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_amdgcn_workitem_id_x() >> 6);
+  const uint32_t unit = wave / (uint32_t)p.kv_heads;
+  const int head = (int)(wave - unit * (uint32_t)p.kv_heads);
+  const uint32_t b = unit / groups;
+  if (b >= (uint32_t)p.batch) return;
+  const int at0 = (int)(unit - b * groups) * kRows;
+  const int len = integer_at(p.lens, b, p.lens_i64, p.columns << p.page_log2);
+  const int at = at0 + lane / kLanes;
+  u32x4 xk{}, xv{};
+  if (at < len) {
+    const int64_t from = page_row(p, page_at(p, (int)b, at0 >> p.page_log2), head) + (at & ((1 << p.page_log2) - 1));
+    if constexpr (CODED) {
+      const u32x2 ck = *reinterpret_cast<const u32x2 *>((const uint8_t *)p.k + from * D + lane % kLanes * 8);
+      const u32x2 cv = *reinterpret_cast<const u32x2 *>((const uint8_t *)p.v + from * D + lane % kLanes * 8);
+      const float sk = scale_of(((const uint8_t *)p.k_scale)[from]), sv = scale_of(((const uint8_t *)p.v_scale)[from]);
+      xk = u32x4{widen_codes<F16, false>(ck[0], sk), widen_codes<F16, true>(ck[0], sk), widen_codes<F16, false>(ck[1], sk),
+                 widen_codes<F16, true>(ck[1], sk)};
+      xv = u32x4{widen_codes<F16, false>(cv[0], sv), widen_codes<F16, true>(cv[0], sv), widen_codes<F16, false>(cv[1], sv),
+                 widen_codes<F16, true>(cv[1], sv)};
+    } else {
+      xk = *reinterpret_cast<const u32x4 *>((const uint16_t *)p.k + from * D + lane % kLanes * 8);
+      xv = *reinterpret_cast<const u32x4 *>((const uint16_t *)p.v + from * D + lane % kLanes * 8);
+    }
+  }
+  if (at >= tokens) return;
+  const int64_t to = (((int64_t)b * tokens + at) * p.kv_heads + head) * D + lane % kLanes * 8;
+  *reinterpret_cast<u32x4 *>(k + to) = xk;
+  *reinterpret_cast<u32x4 *>(v + to) = xv;
+#endif
+}
+
+template <int D, bool F16, bool CODED>
+hipError_t write(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) {
+  const int64_t groups = ((int64_t)a.rows * D / 8 + 63) / 64, waves = groups * a.kv_heads, grid = (waves + kWaves - 1) / kWaves;
+  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
+  return Launch<write_pages_kernel<D, F16, CODED>>::run(grid, kWaves * 64, 0, 0, stream, a, (const uint16_t *)k, (const uint16_t *)v);
+}
+template <int D, bool F16, bool CODED>
+hipError_t read(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream) {
+  const int64_t groups = ((int64_t)tokens * D / 8 + 63) / 64, waves = groups * a.batch * a.kv_heads, grid = (waves + kWaves - 1) / kWaves;
+  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
+  return Launch<read_pages_kernel<D, F16, CODED>>::run(grid, kWaves * 64, 0, 0, stream, a, tokens, (uint32_t)groups, (uint16_t *)k, (uint16_t *)v);
+}
+
+// f(D, F16, CODED) of a call.
+template <template <int, bool, bool> class F, typename... A>
+hipError_t of_kind(const PagesArgs &a, A... args) {
+  const bool coded = a.k_scale != nullptr;
+#define SVODK_KIND(D)                                                                                       \
+  if (a.d == D) {                                                                                           \
+    if (a.f16) return coded ? F<D, true, true>::run(a, args...) : F<D, true, false>::run(a, args...);       \
+    return coded ? F<D, false, true>::run(a, args...) : F<D, false, false>::run(a, args...);                \
+  }
+  SVODK_KIND(64) SVODK_KIND(128) SVODK_KIND(256)
+#undef SVODK_KIND
+  return hipErrorInvalidValue;
+}
+template <int D, bool F16, bool CODED>
+struct Write {
+  static hipError_t run(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) { return write<D, F16, CODED>(a, k, v, stream); }
+};
+template <int D, bool F16, bool CODED>
+struct Read {
+  static hipError_t run(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream) {
+    return read<D, F16, CODED>(a, tokens, k, v, stream);
+  }
+};
+
+}  // namespace
+
+bool pages_support(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+hipError_t launch_write_pages(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) { return of_kind<Write>(a, k, v, stream); }
+hipError_t launch_read_pages(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream) {
+  return of_kind<Read>(a, tokens, k, v, stream);
+}
+
+}  // namespace svodk

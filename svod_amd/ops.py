@@ -51,6 +51,10 @@ class _Attn(ctypes.Structure):
     ]
 
 
+class _Pages(ctypes.Structure):
+    _fields_ = [(n, ctypes.POINTER(_Tensor)) for n in ("k", "v", "k_scale", "v_scale", "table", "lens", "starts")]
+
+
 class _Qkv(ctypes.Structure):
     _fields_ = [
         ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
@@ -133,6 +137,15 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.svodk_plan_linear.argtypes = [ctypes.c_int32, i32p, ctypes.c_int32, i64p, ctypes.c_int32, ctypes.c_int64]
     lib.svodk_order_rows.restype = ctypes.c_int
     lib.svodk_order_rows.argtypes = [tp, tp, ctypes.c_void_p]
+    pp, ap = ctypes.POINTER(_Pages), ctypes.POINTER(_Attn)
+    lib.svodk_write_pages.restype = ctypes.c_int
+    lib.svodk_write_pages.argtypes = [tp, tp, pp, ctypes.c_void_p]
+    lib.svodk_read_pages.restype = ctypes.c_int
+    lib.svodk_read_pages.argtypes = [pp, tp, tp, ctypes.c_void_p]
+    lib.svodk_attention_paged.restype = ctypes.c_int
+    lib.svodk_attention_paged.argtypes = [tp, pp, ap, tp, ctypes.c_void_p]
+    lib.svodk_attention_paged_workspace.restype = ctypes.c_int64
+    lib.svodk_attention_paged_workspace.argtypes = [tp, pp, ap]
     lib.svodk_streaming_next_set.restype = ctypes.c_uint32
     lib.svodk_streaming_next_set.argtypes = []
     lib.svodk_tune_streaming.restype = None
@@ -169,8 +182,10 @@ def _calls():
 
         names = ("attention", "attention_noalloc", "attention_packed", "attention_workspace", "heads", "linear", "layer_norm",
                  "add_layer_norm", "rms_norm", "add_rms_norm", "order_rows")
-        _host.bind({"svodk_" + n: ctypes.cast(getattr(lib, "svodk_" + n), ctypes.c_void_p).value for n in names}, OpError,
-                   _finish, tuple(_DTYPES))
+        pages = ("write_pages", "read_pages", "attention_paged", "attention_paged_workspace")
+        addresses = lambda names: {"svodk_" + n: ctypes.cast(getattr(lib, "svodk_" + n), ctypes.c_void_p).value for n in names}
+        _host.bind_pages(addresses(pages))
+        _host.bind(addresses(names), OpError, _finish, tuple(_DTYPES))
         _native = _host
     return _native
 
@@ -342,6 +357,54 @@ def heads(qkv: torch.Tensor, opts: Qkv, out: Optional[Tuple[torch.Tensor, torch.
     """``qkv [B,T,(heads+2·kv_heads)·head_dim]`` → ``(q [B,T,heads,D], k, v [B,T,kv_heads,D])``
     (tk/src/ops/heads.rs:35-37)."""
     return (_native or _calls()).heads(qkv, opts, out, _fresh if POISON else None)
+
+
+@dataclass
+class Pages:
+    """A key/value cache in pages, and a step's place in it.  Not in the reference, whose caches are whole rows (``Cache``).
+
+    ``k`` and ``v`` are pools ``[pages, kv_heads, page, D]`` of the operands' 16-bit type, or of ``torch.float8_e4m3fn`` with
+    ``scales = (k, v)``, ``[pages, kv_heads, page]`` of ``torch.float8_e8m0fnu``: a row stands for its codes times a power of two.
+    ``page`` is a power of two from 16 to 1024, D 64, 128 or 256.
+
+    Sequence b has ``lens[b]`` tokens, its token at position p in row ``p % page`` of page ``table[b, p // page]`` (int32, entries
+    past its pages unused).  The last ``starts[b + 1] - starts[b]`` of them are the step's new ones, rows ``starts[b]`` and on of
+    the step's packed operands.  ``lens`` and ``starts`` are int32 or int64.  What they hold is looked at on the device alone:
+    one object, and one captured graph, serve every step whose operands have as many rows."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    table: torch.Tensor
+    lens: torch.Tensor
+    starts: Optional[torch.Tensor] = None  # read_pages needs none
+    scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+
+
+def write_pages(k: torch.Tensor, v: torch.Tensor, pages: Pages) -> None:
+    """The new tokens' keys and values ``[N, kv_heads, D]`` into their pages, quantised where those hold 8 bits.  Rows of no
+    sequence are left out.  Enqueued on the current stream of ``k``'s device, as every op."""
+    (_native or _calls()).write_pages(k, v, pages)
+
+
+def read_pages(pages: Pages, tokens: int, dtype: Optional[torch.dtype] = None,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Positions ``0 .. tokens - 1`` of every sequence as ``(k, v)`` ``[B, tokens, kv_heads, D]``, zeros past its end: the
+    layout of ``attention``'s keys.  ``dtype``: of rows that are held in 8 bits, bfloat16 unless named."""
+    return (_native or _calls()).read_pages(pages, tokens, dtype, out, _fresh if POISON else None)
+
+
+def attention_paged(q: torch.Tensor, pages: Pages, opts: Optional[Attn] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention`` of the new tokens' queries ``[N, H, D]``, each at its token's position, over the pages of its sequence;
+    returns ``[N, H, D]``.  ``opts``: ``causal`` (a token sees itself: ``write_pages`` comes first), ``window``, ``scale`` and
+    ``splits``.  With ``splits`` ``None`` the device splits the keys of long sequences, by all the lengths: a row's last bits may
+    depend on them.  Rows of no sequence stay as they are in ``out``."""
+    return (_native or _calls()).attention_paged(q, pages, opts, out, workspace, _fresh if POISON else None)
+
+
+def attention_paged_workspace(q: torch.Tensor, pages: Pages, opts: Optional[Attn] = None) -> int:
+    """The bytes of workspace that ``attention_paged`` allocates for such a call, for a program that lends them."""
+    return int((_native or _calls()).attention_paged_workspace(q, pages, opts))
 
 
 class Act(enum.IntEnum):
