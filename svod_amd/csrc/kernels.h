@@ -231,7 +231,7 @@ struct PagedArgs {
   int32_t win_left, win_right;  // as in AttnArgs; win_left < 0 = no window
   float scale;
   int32_t splits;    // key splits a tile: 0 = the device's choice, 1 = none, or as many as named where there are the blocks
-  float *workspace;  // paged_slots(a) * paged_slot_floats(a) floats; null with `splits` 1
+  float *workspace;  // paged_workspace(a) bytes; null with `splits` 1
 };
 // The most query heads a KV head serves: a tile holds whole tokens.
 constexpr int32_t kMostPagedGroup = 128;
@@ -241,6 +241,7 @@ int paged_tile_rows(const PagedArgs &a);
 int64_t paged_slots(const PagedArgs &a);
 int64_t paged_slot_floats(const PagedArgs &a);
 int64_t paged_workgroups(const PagedArgs &a);
+int64_t paged_workspace(const PagedArgs &a);
 hipError_t launch_paged(const PagedArgs &a, hipStream_t stream);
 const char *paged_config(const PagedArgs &a);
 // One head size's kernels each.

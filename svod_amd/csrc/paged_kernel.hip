@@ -42,13 +42,12 @@ namespace {
 // A value that every lane of a wave has, in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-constexpr int kLeastBlocks = 4;  // key blocks a split has at least, where the device chooses
-
 struct PagedParams {
   PagesArgs pages;
   const uint16_t *q;
   uint16_t *o;
   float *parts;
+  int32_t *told;  // behind them: the blocks an item had
   int32_t heads, group;
   uint32_t group_rcp;
   int32_t tokens;  // of a tile: as many as have their group's rows in it
@@ -56,7 +55,8 @@ struct PagedParams {
   int32_t causal, win_left, win_right;
   float scale;
   int32_t splits;       // as in PagedArgs
-  float per_workgroup;  // kv_heads / the workgroups that fill the chip
+  int32_t places;       // workgroups that the chip holds at a time
+  float crowd, states;  // of blocks_an_item(): company's cost, and that of a state of every row, in steps
   int32_t slots;        // partial states there is room for
 };
 
@@ -76,22 +76,69 @@ __device__ __forceinline__ Demand demand_of(const PagedParams &p, int b) {
 }
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 
-// The key blocks an item may have.
+// The greatest of all lanes' values, none below 0.
+__device__ __forceinline__ int most_of_lanes(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));  // row_shr:1
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15 into rows 1 and 3
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31 into rows 2 and 3
+#endif
+  return last_lane(x);
+}
+constexpr int kNoSplits = 0x7fffffff;  // an item's blocks where none is split
+// A tile's splits where an item has `most` blocks.
+__device__ __forceinline__ int splits_of(const PagedParams &p, int blocks, int most) {
+  if (p.splits != 0) return max(1, min(p.splits, blocks));
+  return blocks <= most ? 1 : (blocks + most - 1) / most;
+}
+// The key blocks an item may have: of those that would fill the chip once and up to twice as many, and of the longest tile's,
+// what ends first by this reckoning, in steps of a block.  Items run a round of the chip's places at a time, a step of four waves
+// with company on its compute unit takes `crowd` times one's alone; an item starts in kStart steps (the deal, the pages,
+// the first blocks: trips to memory); a call that splits writes its rows' states, reads them and has its merge behind it.
+// (By the blocks of all items over the places alone 16 sequences over 210 to 2100 keys were 528 items on 512 places, 22.9 us for 19.4;
+// without the states two chunks of 1001 rows in a window of 1024 split in two, 46 us for 32.)
+constexpr int kLeastBlocks = 2, kStart = 3, kMerge = 3;
 __device__ __forceinline__ int blocks_an_item(const PagedParams &p, const Demand &first) {
-  if (p.splits != 0) return 0;
-  int high = 0, low = 0;
+  if (p.splits != 0) return kNoSplits;
+  constexpr int kTries = 4, kQuarters[kTries] = {4, 5, 6, 8};
+  int high = 0, low = 0, longest = 0, tiles = 0;
   const int lane = (int)__builtin_amdgcn_workitem_id_x() & 63;
   for (int base = 0; base < p.pages.batch; base += 64) {
     const Demand d = base == 0 ? first : demand_of(p, base + lane);
     const int64_t work = (int64_t)d.tiles * d.blocks;
     high += (int)(work >> 12), low += (int)(work & 4095);
+    longest = max(longest, d.tiles > 0 ? d.blocks : 0);
+    tiles += d.tiles;
   }
-  const float total = (float)last_lane(sum_to_lane(high)) * 4096.0f + (float)last_lane(sum_to_lane(low));
-  return max(kLeastBlocks, (int)__builtin_ceilf(total * p.per_workgroup));
-}
-__device__ __forceinline__ int splits_of(const PagedParams &p, int blocks, int most) {
-  if (p.splits != 0) return max(1, min(p.splits, blocks));
-  return blocks <= most ? 1 : (blocks + most - 1) / most;
+  const float heads = (float)p.pages.kv_heads, places = (float)p.places, all_tiles = (float)last_lane(sum_to_lane(tiles));
+  const float blocks = ((float)last_lane(sum_to_lane(high)) * 4096.0f + (float)last_lane(sum_to_lane(low))) * heads;
+  longest = most_of_lanes(longest);
+  const float a_place = __builtin_amdgcn_rcpf(places), a_tile = __builtin_amdgcn_rcpf(all_tiles);
+  const int once = max(kLeastBlocks, (int)__builtin_ceilf(blocks / places));
+  int sums[kTries] = {};
+  for (int base = 0; base < p.pages.batch; base += 64) {
+    const Demand d = base == 0 ? first : demand_of(p, base + lane);
+#pragma unroll
+    for (int i = 0; i < kTries; i++) sums[i] += d.tiles * splits_of(p, d.blocks, (once * kQuarters[i] + 3) / 4);
+  }
+  auto time_of = [&](float items, int most) {
+    const float alone = (float)most * (2.0f * items > places ? p.crowd : 1.0f) + (float)kStart;
+    if (items <= places) return alone;
+    return __builtin_fmaxf(alone, __builtin_ceilf(items * a_place) * (blocks * __builtin_amdgcn_rcpf(items) * p.crowd + (float)kStart));
+  };
+  int best = kNoSplits;
+  float best_time = time_of(all_tiles * heads, longest);
+#pragma unroll
+  for (int i = kTries - 1; i >= 0; i--) {
+    const int most = (once * kQuarters[i] + 3) / 4;
+    const float items = (float)last_lane(sum_to_lane(sums[i]));
+    const float time = time_of(items * heads, most) + (float)kMerge + p.states * items * a_tile;
+    if (most < longest && time < best_time) best = most, best_time = time;
+  }
+  return best;
 }
 
 // Where an item, or a row, is in the deal.
@@ -143,9 +190,10 @@ __device__ __forceinline__ Place place_of(const PagedParams &p, int item, const 
 
 // ---- keys in pages.  A fill instruction moves 1 KiB, 16 bytes a lane: whole rows of one KV head, 16 of which never lie in two
 // pages.  So a wave's fills of a block go by runs of 16 rows, with a page looked up and a descriptor made for each.
-template <int D, int NW, bool CODED>
-struct Pages<D, NW, true, CODED> {
-  static constexpr int kRowBytes = CODED ? D : 2 * D;
+template <int D, int NW, unsigned FLAGS>
+struct PagesOf {
+  static constexpr bool kCodes = (FLAGS & kCoded) != 0, kStages = (FLAGS & kStaged) != 0;
+  static constexpr int kRowBytes = kCodes ? D : 2 * D;
   static constexpr int kLanes = kRowBytes / 16;          // lanes a row
   static constexpr int kRows = 64 / kLanes;              // rows a fill
   static constexpr int kFills = kBkv / kRows / NW;       // a wave's fills of a tile, kStride rows apart
@@ -163,11 +211,11 @@ struct Pages<D, NW, true, CODED> {
   int column, ids, ids_next;
   int64_t run[kRuns];                // the pool's row that each of this wave's runs of the block filled last starts at
   int run_row;                       // the first run's row of the block
-  int k_src[kPer], v_src[kPer];      // a lane's offset in a run's descriptor (16-bit keys: swizzled)
-  int k_dst[kPer], v_dst[kPer];      // where its codes go in a slot, widened: these 16 bytes and the ones at ^ 16
+  int k_src[kPer], v_src[kPer];      // a lane's offset in a run's descriptor (straight into LDS: swizzled)
+  int k_dst[kPer], v_dst[kPer];      // where its 16 bytes go in a slot; of codes, widened, the second 16 go to ^ 16
   struct Stage {
-    u32x4 codes[CODED ? kFills : 1];
-    uint32_t scale[CODED ? kFills : 1];
+    u32x4 rows[kStages ? kFills : 1];
+    uint32_t scale[kCodes ? kFills : 1];
   };
   Stage k_stage, v_stage;
 
@@ -197,20 +245,26 @@ struct Pages<D, NW, true, CODED> {
     }
   }
 };
+template <int D, int NW>
+struct Pages<D, NW, kPaged> : PagesOf<D, NW, kPaged> {};
+template <int D, int NW>
+struct Pages<D, NW, kPaged | kStaged> : PagesOf<D, NW, kPaged | kStaged> {};
+template <int D, int NW>
+struct Pages<D, NW, kPaged | kStaged | kCoded> : PagesOf<D, NW, kPaged | kStaged | kCoded> {};
 
 // A descriptor over `rows` rows of `row_bytes` at `base`: rows from there on read as zeros.
-__device__ __forceinline__ i32x4 rows_rsrc(const uint8_t *base, int rows, int row_bytes) {
+[[maybe_unused]] __device__ __forceinline__ i32x4 rows_rsrc(const uint8_t *base, int rows, int row_bytes) {
   const uint64_t at = (uint64_t)(uintptr_t)base;
   // The same in every lane, and told so: a 64-bit sum that the compiler has on the VALU is no scalar to it.
   return i32x4{uniform((int)(uint32_t)at), uniform((int)(uint32_t)(at >> 32)), uniform(rows * row_bytes), 0x00020000};
 }
 
-// This wave's share of block `n` from the pool at `base`, whose runs find() has named: keys past the length land as zeros (a
-// page's last rows hold anything, and 0 times that is not 0).
+// This wave's share of block `n` from the pool at `base`, whose runs find() has named, straight into LDS: keys past the length
+// land as zeros (a page's last rows hold anything, and 0 times that is not 0).
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_pages(const Wave<D, NW, F16, FLAGS> &w, const uint8_t *base, int n, int lds_at,
                                            const int *src) {
-  using P = Pages<D, NW, true, false>;
+  using P = decltype(w.pages);
 #pragma unroll
   for (int r = 0; r < P::kRuns; r++) {
     const int left = min(max(w.len - n * kBkv - w.pages.row_of(r), 0), 16);
@@ -223,47 +277,54 @@ __device__ __forceinline__ void fill_pages(const Wave<D, NW, F16, FLAGS> &w, con
                    : "memory");
   }
 }
-// The same of codes: into registers, with their rows' scales.
-template <int D, int NW, bool F16, unsigned FLAGS>
+// The same into registers, codes with their rows' scales.
+template <int D, int NW, bool F16, unsigned FLAGS, typename S>
 __device__ __forceinline__ void stage_pages(const Wave<D, NW, F16, FLAGS> &w, const uint8_t *base, const uint8_t *scales, int n,
-                                            const int *src, typename Pages<D, NW, true, true>::Stage &stage) {
+                                            const int *src, S &stage) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using P = Pages<D, NW, true, true>;
+  using P = decltype(w.pages);
 #pragma unroll
   for (int r = 0; r < P::kRuns; r++) {
     const int left = min(max(w.len - n * kBkv - w.pages.row_of(r), 0), 16);
-    const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + w.pages.run[r] * D), 0, left * D, 0x00020000);
-    const auto scale = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(scales + w.pages.run[r]), 0, left, 0x00020000);
+    const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + w.pages.run[r] * P::kRowBytes), 0,
+                                                        left * P::kRowBytes, 0x00020000);
 #pragma unroll
-    for (int j = 0; j < P::kPer; j++) {
-      stage.codes[r * P::kPer + j] = __builtin_amdgcn_raw_buffer_load_b128(codes, src[j], 0, 0);
-      stage.scale[r * P::kPer + j] = __builtin_amdgcn_raw_buffer_load_b8(scale, src[j] / D, 0, 0);
+    for (int j = 0; j < P::kPer; j++) stage.rows[r * P::kPer + j] = __builtin_amdgcn_raw_buffer_load_b128(rows, src[j], 0, 0);
+    if constexpr (P::kCodes) {
+      const auto scale = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(scales + w.pages.run[r]), 0, left, 0x00020000);
+#pragma unroll
+      for (int j = 0; j < P::kPer; j++)
+        stage.scale[r * P::kPer + j] = __builtin_amdgcn_raw_buffer_load_b8(scale, src[j] / P::kRowBytes, 0, 0);
     }
   }
 #endif
 }
-// And from there, widened, into a slot.
-template <int D, int NW, bool F16>
-__device__ __forceinline__ void land_stage(uint8_t *slot, const int *dst, const typename Pages<D, NW, true, true>::Stage &stage) {
-  using P = Pages<D, NW, true, true>;
+// And from there into a slot.
+template <int D, int NW, bool F16, unsigned FLAGS, typename S>
+__device__ __forceinline__ void land_stage(const Wave<D, NW, F16, FLAGS> &w, uint8_t *slot, const int *dst, const S &stage) {
+  using P = decltype(w.pages);
 #pragma unroll
   for (int i = 0; i < P::kFills; i++) {
-    const float scale = scale_of(stage.scale[i]);
-    const u32x4 c = stage.codes[i];
+    const u32x4 c = stage.rows[i];
     uint8_t *at = slot + (i - i % P::kPer) * P::kStride * Tile<D>::kRowBytes;
-    const u32x4 lo = {widen_codes<F16, false>(c[0], scale), widen_codes<F16, true>(c[0], scale),
-                      widen_codes<F16, false>(c[1], scale), widen_codes<F16, true>(c[1], scale)};
-    const u32x4 hi = {widen_codes<F16, false>(c[2], scale), widen_codes<F16, true>(c[2], scale),
-                      widen_codes<F16, false>(c[3], scale), widen_codes<F16, true>(c[3], scale)};
-    *reinterpret_cast<u32x4 *>(at + dst[i % P::kPer]) = lo;
-    *reinterpret_cast<u32x4 *>(at + (dst[i % P::kPer] ^ 16)) = hi;
+    if constexpr (P::kCodes) {
+      const float scale = scale_of(stage.scale[i]);
+      const u32x4 lo = {widen_codes<F16, false>(c[0], scale), widen_codes<F16, true>(c[0], scale),
+                        widen_codes<F16, false>(c[1], scale), widen_codes<F16, true>(c[1], scale)};
+      const u32x4 hi = {widen_codes<F16, false>(c[2], scale), widen_codes<F16, true>(c[2], scale),
+                        widen_codes<F16, false>(c[3], scale), widen_codes<F16, true>(c[3], scale)};
+      *reinterpret_cast<u32x4 *>(at + dst[i % P::kPer]) = lo;
+      *reinterpret_cast<u32x4 *>(at + (dst[i % P::kPer] ^ 16)) = hi;
+    } else {
+      *reinterpret_cast<u32x4 *>(at + dst[i % P::kPer]) = c;
+    }
   }
 }
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
   if (n >= w.end) return;
   w.pages.find(n);
-  if constexpr ((FLAGS & kCoded) != 0)
+  if constexpr ((FLAGS & kStaged) != 0)
     stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n, w.pages.k_src, w.pages.k_stage);
   else
     fill_pages<D, NW>(w, w.k_base, n, w.lds0 + slot * Tile<D>::kBytes, w.pages.k_src);
@@ -272,7 +333,7 @@ __device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, 
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
   if (n >= w.end) return;
-  if constexpr ((FLAGS & kCoded) != 0)
+  if constexpr ((FLAGS & kStaged) != 0)
     stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n, w.pages.v_src, w.pages.v_stage);
   else
     fill_pages<D, NW>(w, w.v_base, n, w.lds0 + (2 + slot) * Tile<D>::kBytes, w.pages.v_src);
@@ -280,15 +341,22 @@ __device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, 
 // The end of step `blk`: what its fills asked for goes into the ring, V(blk + 1) and K(blk + 2).
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void land_pages(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk, int par) {
-  if (blk + 1 < w.end) land_stage<D, NW, F16>(smem + (2 + (par ^ 1)) * Tile<D>::kBytes, w.pages.v_dst, w.pages.v_stage);
-  if (blk + 2 < w.end) land_stage<D, NW, F16>(smem + par * Tile<D>::kBytes, w.pages.k_dst, w.pages.k_stage);
+  if (blk + 1 < w.end) land_stage<D, NW>(w, smem + w.v_slot(par ^ 1) * Tile<D>::kBytes, w.pages.v_dst, w.pages.v_stage);
+  if (blk + 2 < w.end) land_stage<D, NW>(w, smem + w.k_slot(par) * Tile<D>::kBytes, w.pages.k_dst, w.pages.k_stage);
 }
+
+// Whether a form's tiles come through registers: codes, which are widened there; and the keys of a wave by itself, which then
+// needs one slot for them and one for values, half the LDS, so that a compute unit holds twice the waves (at D 256 the
+// registers do not hold a tile).
+template <int D, int NW, bool CODED>
+constexpr bool kStages = CODED || (NW == 1 && D <= 128);
 
 template <int D, int NW, bool F16, bool CODED>
 __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) {
   using TL = Tile<D>;
-  using W = Wave<D, NW, F16, kRanged | kPaged | (CODED ? kCoded : 0u)>;
-  using P = Pages<D, NW, true, CODED>;
+  constexpr bool kThroughRegisters = kStages<D, NW, CODED>;
+  using W = Wave<D, NW, F16, kRanged | kPaged | (kThroughRegisters ? kStaged : 0u) | (CODED ? kCoded : 0u)>;
+  using P = decltype(W::pages);
   constexpr int BQ = NW * kWaveRows, KS = W::KS, DB = W::DB;
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
   W w;
@@ -304,6 +372,8 @@ __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) 
   const Demand first_demand = demand_of(p, w.lane);
   const int most = blocks_an_item(p, first_demand);
   const Place at = place_of<false>(p, item, first_demand, most);
+  // The merge goes by the same deal: it is told what this launch went by, behind the states.
+  if (wg == 0 && tid == 0 && p.slots > 0) *p.told = most;
   if (!at.found) return;
   const int slot = (at.slot + at.split) * p.pages.kv_heads + kvh;
   if (at.splits > 1 && slot >= p.slots) return;  // lengths that are none: more rows than there are
@@ -382,11 +452,11 @@ __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) 
 #pragma unroll
   for (int j = 0; j < P::kPer; j++) {
     const int in_run = ((w.wave * P::kRows) & 15) + j * P::kStride + w.lane / P::kLanes, pc = w.lane % P::kLanes;
-    if constexpr (CODED) {
+    if constexpr (kThroughRegisters) {
       w.pages.k_src[j] = w.pages.v_src[j] = in_run * P::kRowBytes + pc * 16;
-      const int r = w.wave * P::kRows + j * P::kStride + w.lane / P::kLanes;
-      w.pages.k_dst[j] = r * TL::kRowBytes + (((2 * pc) ^ TL::swz_k(r)) << 4);
-      w.pages.v_dst[j] = r * TL::kRowBytes + (((2 * pc) ^ (TL::swz_v(r) << 2)) << 4);
+      const int r = w.wave * P::kRows + j * P::kStride + w.lane / P::kLanes, chunk = CODED ? 2 * pc : pc;
+      w.pages.k_dst[j] = r * TL::kRowBytes + ((chunk ^ TL::swz_k(r)) << 4);
+      w.pages.v_dst[j] = r * TL::kRowBytes + ((chunk ^ (TL::swz_v(r) << 2)) << 4);
     } else {
       w.pages.k_src[j] = in_run * P::kRowBytes + ((pc ^ TL::swz_k(in_run)) << 4);
       w.pages.v_src[j] = in_run * P::kRowBytes + ((pc ^ (TL::swz_v(in_run) << 2)) << 4);
@@ -401,8 +471,8 @@ __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) 
     if (row_ok) x = *reinterpret_cast<const u32x4 *>(q_ptr + ks * 16);
     w.qf[ks] = x;
   }
-  if constexpr (CODED) {
-    typename P::Stage ahead;
+  typename P::Stage ahead;
+  if constexpr (kThroughRegisters) {
     fill_k<D, NW>(w, 0, 0);
     fill_v<D, NW>(w, 0, 0);
     if (end > 1) {
@@ -410,10 +480,10 @@ __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) 
       stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, 1, w.pages.k_src, ahead);
     }
     if (end > 0) {
-      land_stage<D, NW, F16>(smem, w.pages.k_dst, w.pages.k_stage);
-      land_stage<D, NW, F16>(smem + 2 * TL::kBytes, w.pages.v_dst, w.pages.v_stage);
+      land_stage<D, NW>(w, smem, w.pages.k_dst, w.pages.k_stage);
+      land_stage<D, NW>(w, smem + W::v_slot(0) * TL::kBytes, w.pages.v_dst, w.pages.v_stage);
     }
-    if (end > 1) land_stage<D, NW, F16>(smem + TL::kBytes, w.pages.k_dst, ahead);
+    if (!W::kOneSlot && end > 1) land_stage<D, NW>(w, smem + TL::kBytes, w.pages.k_dst, ahead);
   } else {
     fill_k<D, NW>(w, 0, 0);
     fill_v<D, NW>(w, 0, 0);
@@ -460,6 +530,9 @@ __device__ __forceinline__ void paged_body(uint8_t *smem, const PagedParams &p) 
     seen = halves_seen<D, NW, false>(w, 0, kbits0);
     if (on_edge<D, NW, false>(w, 0, kbits0)) mask_scores<D, NW, false>(w, 0, kbits0, sv);
     bm = row_max(sv);
+  }
+  if constexpr (W::kOneSlot) {
+    if (end > 1) land_stage<D, NW>(w, smem, w.pages.k_dst, ahead);
   }
   __syncthreads();  // step 0 refills the K slot those scores were read from
   int full = 0;
@@ -523,73 +596,92 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : (D <= 128 ? 2 : 1)) void pag
 #endif
 }
 
-// The rows of split tiles: each the sum of its splits' states under their common maximum, in the order of the splits.  A wave
-// a (row, head) at a time, `run` of them one after the other; a call whose deal splits nothing leaves at once.
+// The rows of split tiles: each the sum of its splits' states under their common maximum.  A workgroup takes `run` pieces of a
+// packed row one after the other, a piece as many heads as a wave has lanes for at eight columns each; its waves take the
+// splits in turn, eight states asked for at a time with their maxima (one trip to memory for 32 splits), and the first wave adds up what they
+// have, in their order.  A launch that split nothing leaves at once.
+template <int D>
+constexpr int kMergeHeads = 512 / D;
 template <int D, int BQ, bool F16>
 __global__ __launch_bounds__(256) void merge_kernel(PagedParams p, int run) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int E = D / 64;  // columns a lane
-  constexpr int kAhead = 8;
+  constexpr int kLanes = D / 8, kAhead = 8;
+  __shared__ __attribute__((aligned(16))) f32x4 of_waves[3][64][3];
+  const int most = uniform(*p.told);
+  if (most == kNoSplits && p.splits == 0) return;
   const int lane = (int)__builtin_amdgcn_workitem_id_x() & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)__builtin_amdgcn_workitem_id_x() >> 6);
+  const int wave = uniform((int)__builtin_amdgcn_workitem_id_x() >> 6);
   const Demand first_demand = demand_of(p, lane);
-  const int most = blocks_an_item(p, first_demand);
-  const int64_t from = ((int64_t)__builtin_amdgcn_workgroup_id_x() * 4 + wave) * run;
+  const uint32_t pieces = (uint32_t)(p.heads + kMergeHeads<D> - 1) / kMergeHeads<D>;
+  const uint32_t from = (uint32_t)__builtin_amdgcn_workgroup_id_x() * (uint32_t)run;
+  int row = (int)(from / pieces), piece = (int)(from - (uint32_t)row * pieces), known = -1;
   Place at{};
-  int known = -1;
-  int row = (int)((uint32_t)from / (uint32_t)p.heads), head = (int)from - row * p.heads;  // (row, head)s are fewer than 2^31
-  for (int i = 0; i < run && row < p.pages.rows; i++, head = head + 1 < p.heads ? head + 1 : 0, row += head == 0 ? 1 : 0) {
+  for (int i = 0; i < run && row < p.pages.rows; i++) {
     if (row != known) at = place_of<true>(p, row, first_demand, most);
     known = row;
-    if (!at.found || at.splits <= 1) continue;
-    const int kvh = (int)div_by((uint32_t)head, (uint32_t)p.group, p.group_rcp);
-    const int in_tile = (row - at.s.start - at.tile * p.tokens) * p.group + head - kvh * p.group;
-    const int64_t step = (int64_t)p.pages.kv_heads * (BQ * (D + 2));
-    if ((int64_t)(at.slot + at.splits - 1) * p.pages.kv_heads + kvh >= p.slots) continue;  // as paged_body
-    const float *part = p.parts + ((int64_t)at.slot * p.pages.kv_heads + kvh) * (BQ * (D + 2));
-    float m = -INFINITY;
-    for (int s = lane; s < at.splits; s += 64) m = __builtin_fmaxf(m, part[s * step + BQ * D + in_tile]);
+    const int head = piece * kMergeHeads<D> + lane / kLanes, here = min(head, p.heads - 1);
+    const int kvh = (int)div_by((uint32_t)here, (uint32_t)p.group, p.group_rcp);
+    const int last = at.splits - 1;
+    // (Slots past the workspace's: as paged_body.  The branch is the same in all waves.)
+    if (at.found && last > 0 && (int64_t)(at.slot + last + 1) * p.pages.kv_heads <= p.slots) {
+      const int in_tile = (row - at.s.start - at.tile * p.tokens) * p.group + here - kvh * p.group;
+      const int64_t step = (int64_t)p.pages.kv_heads * (BQ * (D + 2));
+      const float *part = p.parts + ((int64_t)at.slot * p.pages.kv_heads + kvh) * (BQ * (D + 2));
+      const int column = lane % kLanes * 8;
+      float m = -1e30f, l = 0.0f, acc[8] = {};
+      for (int base = wave * kAhead; base <= last; base += 4 * kAhead) {
+        f32x4 x[kAhead][2];
+        float ms[kAhead], ls[kAhead];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off));
-    float acc[E], l = 0.0f;
+        for (int j = 0; j < kAhead; j++) {  // one past the last asks for the last again, and weighs nothing
+          const float *state = part + min(base + j, last) * step;
+          ms[j] = state[BQ * D + in_tile];
+          ls[j] = state[BQ * D + BQ + in_tile];
+          x[j][0] = *reinterpret_cast<const f32x4 *>(state + in_tile * D + column);
+          x[j][1] = *reinterpret_cast<const f32x4 *>(state + in_tile * D + column + 4);
+        }
+        float top = m;
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = 0.0f;
-    for (int base_s = 0; base_s < at.splits; base_s += 64) {
-      float weight = 0.0f, sum = 0.0f;
-      if (base_s + lane < at.splits) {
-        const float *state = part + (base_s + lane) * step + BQ * D + in_tile;
-        weight = fast_exp2(state[0] - m);
-        sum = state[BQ] * weight;
-      }
+        for (int j = 0; j < kAhead; j++) top = __builtin_fmaxf(top, ms[j]);
+        const float keep = fast_exp2(m - top);
+        m = top;
+        l *= keep;
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-      l += sum;
-      const int here = min(64, at.splits - base_s);
-      for (int s = 0; s < here; s += kAhead) {
-        // Eight states' loads in flight; one past the last loads the last and weighs nothing.
-        float x[kAhead][E];
+        for (int e = 0; e < 8; e++) acc[e] *= keep;
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-          const float *from_state = part + (base_s + min(s + j, here - 1)) * step + in_tile * D + lane * E;
+          const float weight = base + j <= last ? fast_exp2(ms[j] - top) : 0.0f;
+          l = __builtin_fmaf(ls[j], weight, l);
 #pragma unroll
-          for (int e = 0; e < E; e++) x[j][e] = from_state[e];
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; j++) {
-          const float wt = s + j < here ? __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(weight), s + j)) : 0.0f;
-#pragma unroll
-          for (int e = 0; e < E; e++) acc[e] = __builtin_fmaf(x[j][e], wt, acc[e]);
+          for (int e = 0; e < 8; e++) acc[e] = __builtin_fmaf(x[j][e / 4][e % 4], weight, acc[e]);
         }
       }
-    }
-    const float inv = 1.0f / (l == 0.0f ? 1.0f : l);
-    uint16_t *out = p.o + ((int64_t)row * p.heads + head) * D + lane * E;
-    if constexpr (E == 1) {
-      *out = (uint16_t)pack2<F16>(acc[0] * inv, 0.0f);
-    } else {
+      const int waves = min(4, last / kAhead + 1);  // that had splits
+      if (waves > 1) {
+        __syncthreads();  // the piece before has been read
+        if (wave > 0) {
+          of_waves[wave - 1][lane][0] = f32x4{m, l, 0.0f, 0.0f};
+          of_waves[wave - 1][lane][1] = f32x4{acc[0], acc[1], acc[2], acc[3]};
+          of_waves[wave - 1][lane][2] = f32x4{acc[4], acc[5], acc[6], acc[7]};
+        }
+        __syncthreads();
+        for (int o = 1; o < waves; o++) {
+          const f32x4 ml = of_waves[o - 1][lane][0], x0 = of_waves[o - 1][lane][1], x1 = of_waves[o - 1][lane][2];
+          const float top = __builtin_fmaxf(m, ml[0]), keep = fast_exp2(m - top), weight = fast_exp2(ml[0] - top);
+          m = top;
+          l = l * keep + ml[1] * weight;
 #pragma unroll
-      for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = pack2<F16>(acc[e] * inv, acc[e + 1] * inv);
+          for (int e = 0; e < 8; e++) acc[e] = acc[e] * keep + (e < 4 ? x0[e % 4] : x1[e % 4]) * weight;
+        }
+      }
+      const float inv = 1.0f / (l == 0.0f ? 1.0f : l);
+      u32x4 out;
+#pragma unroll
+      for (int e = 0; e < 4; e++) out[e] = pack2<F16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      if (wave == 0 && head < p.heads) *reinterpret_cast<u32x4 *>(p.o + ((int64_t)row * p.heads + head) * D + column) = out;
     }
+    piece++;
+    if (piece == (int)pieces) piece = 0, row++;
   }
 #endif
 }
@@ -597,13 +689,16 @@ __global__ __launch_bounds__(256) void merge_kernel(PagedParams p, int run) {
 // ---- the launch.
 constexpr int kUnits = 256;  // compute units of an MI355X
 // Workgroups of a form that a compute unit holds: by their rings' LDS, of 160 KiB, and for four waves by their registers.
-template <int D, int NW>
-constexpr int kResident = NW == 1 ? (160 * 1024 / Tile<D>::kLds < 4 ? 160 * 1024 / Tile<D>::kLds : 4) : (D <= 128 ? 2 : 1);
+template <int D, int NW, bool CODED>
+constexpr int kRing = NW == 1 && kStages<D, NW, CODED> ? 2 * Tile<D>::kBytes : Tile<D>::kLds;
+constexpr int least(int a, int b) { return a < b ? a : b; }
+template <int D, int NW, bool CODED>
+constexpr int kResident = NW == 1 ? least(160 * 1024 / kRing<D, NW, CODED>, D == 64 ? 8 : 4) : (D <= 128 ? 2 : 1);
 
-uint32_t rcp_of(uint32_t d) { return d <= 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / d); }
+[[maybe_unused]] uint32_t rcp_of(uint32_t d) { return d <= 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / d); }
 
 // Tiles there may be, of one KV head: every sequence's last may be short, and none is empty.
-int64_t tiles_at_most(const PagedArgs &a) {
+[[maybe_unused]] int64_t tiles_at_most(const PagedArgs &a) {
   const int64_t tokens = paged_tile_rows(a) / (a.heads / a.pages.kv_heads), rows = a.pages.rows;
   return rows < rows / tokens + a.pages.batch ? rows : rows / tokens + a.pages.batch;
 }
@@ -626,16 +721,18 @@ hipError_t launch(const PagedArgs &a, hipStream_t stream) {
   p.win_right = a.win_right;
   p.scale = a.scale;
   p.splits = a.splits;
-  const int64_t filled = (int64_t)kUnits * kResident<D, NW>;
-  p.per_workgroup = (float)a.pages.kv_heads / (float)filled;
+  p.places = kUnits * kResident<D, NW, CODED>;
+  p.crowd = NW == 1 ? 1.0f : 1.25f;
+  p.states = (float)((double)a.pages.rows * a.heads * (D + 2) * 8 / 7e6);  // written and read at 5 MB a us, 1.4 us a step
   const int64_t slots = paged_slots(a);
   p.slots = (int32_t)slots;
+  p.told = reinterpret_cast<int32_t *>(p.parts + slots * paged_slot_floats(a));
   const int64_t grid = paged_workgroups(a);
-  hipError_t e = Launch<paged_kernel<D, NW, F16, CODED>>::run(grid, NW * 64, Tile<D>::kLds, Tile<D>::kLds, stream, p);
+  hipError_t e = Launch<paged_kernel<D, NW, F16, CODED>>::run(grid, NW * 64, kRing<D, NW, CODED>, kRing<D, NW, CODED>, stream, p);
   if (e != hipSuccess || slots == 0) return e;
-  const int64_t rows = (int64_t)a.pages.rows * a.heads, waves = (int64_t)kUnits * 32;
-  const int run = (int)((rows + waves - 1) / waves);
-  return Launch<merge_kernel<D, BQ, F16>>::run((rows + 4ll * run - 1) / (4ll * run), 256, 0, 0, stream, p, run);
+  const int64_t pieces = (int64_t)a.pages.rows * ((a.heads + kMergeHeads<D> - 1) / kMergeHeads<D>), at_once = (int64_t)kUnits * 8;
+  const int run = (int)((pieces + at_once - 1) / at_once);
+  return Launch<merge_kernel<D, BQ, F16>>::run((pieces + run - 1) / run, 256, 0, 0, stream, p, run);
 }
 
 template <int D>
@@ -670,6 +767,11 @@ int64_t paged_workgroups(const PagedArgs &a) {
   return a.splits > 1 ? tiles * a.splits : tiles + paged_slots(a);
 }
 
+int64_t paged_workspace(const PagedArgs &a) {
+  const int64_t slots = paged_slots(a);
+  return slots == 0 ? 0 : slots * paged_slot_floats(a) * 4 + 16;
+}
+
 int64_t paged_slot_floats(const PagedArgs &a) { return (int64_t)paged_tile_rows(a) * (a.pages.d + 2); }
 
 int64_t paged_slots(const PagedArgs &a) {
@@ -679,8 +781,11 @@ int64_t paged_slots(const PagedArgs &a) {
   // A tile of b blocks is split where b > n, the blocks an item may have, into fewer than 2 b / n: over all tiles fewer than
   // twice what fills the chip.  (And 2 for n's rounding.)
   if (blocks <= kLeastBlocks) return 0;
-  const int resident = paged_tile_rows(a) == 32 ? (a.pages.d == 64 ? kResident<64, 1> : a.pages.d == 128 ? kResident<128, 1> : kResident<256, 1>)
-                                                : (a.pages.d <= 128 ? 2 : 1);
+  const bool coded = a.pages.k_scale != nullptr;
+  const int resident = paged_tile_rows(a) != 32 ? (a.pages.d <= 128 ? 2 : 1)
+                       : a.pages.d == 64        ? (coded ? kResident<64, 1, true> : kResident<64, 1, false>)
+                       : a.pages.d == 128       ? (coded ? kResident<128, 1, true> : kResident<128, 1, false>)
+                                                : (coded ? kResident<256, 1, true> : kResident<256, 1, false>);
   return 2ll * kUnits * resident + 2;
 }
 

@@ -237,7 +237,7 @@ int svodk_attention_paged(const svodk_tensor *q, const svodk_pages *pages, const
   int n = 2;
   if (a.splits != 1) {
     // Splits that the caller named need their workspace; the device's own are dropped without it.
-    const int64_t need = svodk::paged_slots(a) * svodk::paged_slot_floats(a) * 4;
+    const int64_t need = svodk::paged_workspace(a);
     const bool lent = opts->workspace != nullptr && opts->workspace_bytes >= need;
     if (!lent && a.splits > 1) return ran_graph(op, SVODK_GRAPH_CONFIG);
     if (!lent) {
@@ -259,7 +259,7 @@ int64_t svodk_attention_paged_workspace(const svodk_tensor *q, const svodk_pages
   svodk::PagedArgs a{};
   int why;
   if (take_paged(q, pages, opts, a, why) != 0 || why != 0 || a.splits == 1) return 0;
-  return svodk::paged_slots(a) * svodk::paged_slot_floats(a) * 4;
+  return svodk::paged_workspace(a);
 }
 
 }  // extern "C"
