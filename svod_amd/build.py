@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsvodk_gfx950.so")
 HOST = os.path.join(HERE, "_host.so")  # the Python side's calls (csrc/host.cpp), a module of this package
 SOURCES = ["ops.cpp", "pages.cpp", "heads_kernel.hip", "attention_kernel.hip", "combine_kernel.hip", "rows_kernel.hip",
-           "linear_kernel.hip", "linear_few_kernel.hip", "decode_kernel.hip", "pages_kernel.hip", "paged_kernel.hip"]
+           "linear_kernel.hip", "linear_few_kernel.hip", "decode_kernel.hip", "pages_kernel.hip", "paged_kernel.hip", "paged_few_kernel.hip"]
 
 # Packed-FP32 VALU ops are switched off for device code; the host pass of hipcc
 # does not know the feature and says so, which is harmless.
@@ -32,7 +32,9 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang"
 # rewrite for wave-uniform operands waits for the answer where the add is issued.
 EXTRA_FLAGS = {"attention_kernel.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-kernarg-preload-count=16",
                                         "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
-               "paged_kernel.hip": ["-fno-honor-nans"]}  # the same steps
+               # The same steps, and a wave's deal of the launch's work asks for its arguments first.
+               "paged_kernel.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-kernarg-preload-count=13"],
+               "paged_few_kernel.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-kernarg-preload-count=13"]}
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-command-line-argument"]
 
 

@@ -157,8 +157,7 @@ constexpr unsigned kRanged = 2;  // per-row key ranges: window, chunk mask, segm
 constexpr unsigned kBiased = 4;  // an additive bias joins the scaled scores
 constexpr unsigned kSided = 8;   // one of a tile's two sides: every other key block is this wave's
 constexpr unsigned kPaged = 16;  // the keys lie in pages
-constexpr unsigned kStaged = 32; // and come into the ring through registers
-constexpr unsigned kCoded = 64;  // as e4m3 codes, which are widened there
+constexpr unsigned kCoded = 32;  // as e4m3 codes, which come into the ring through registers and are widened there
 
 // What a wave knows of its keys' pages: nothing where they lie in rows.
 template <int D, int NW, unsigned FLAGS>
@@ -220,13 +219,8 @@ struct Wave {
   const uint8_t *nxt_k, *nxt_v;
   int64_t nxt_bytes;
   int nxt_end, end_even;
-  // The ring's slots of a block of parity `par`.  A wave by itself whose tiles come through registers has one for keys and one
-  // for values: it writes a tile when it has read the one before.
-  static constexpr bool kOneSlot = (FLAGS & kStaged) != 0 && NW == 1;
-  __device__ static constexpr int k_slot(int par) { return kOneSlot ? 0 : par; }
-  __device__ static constexpr int v_slot(int par) { return kOneSlot ? 1 : 2 + par; }
   // Keys in pages (paged_kernel.hip's fills).
-  Pages<D, NW, FLAGS & (kPaged | kStaged | kCoded)> pages;
+  Pages<D, NW, FLAGS & (kPaged | kCoded)> pages;
 };
 
 // A tile's fills where its keys lie in pages: defined beside Pages.
@@ -551,8 +545,8 @@ __device__ __forceinline__ void hot_step(Wave<D, NW, F16, FLAGS> &w, const uint8
   constexpr int KS = Wave<D, NW, F16, FLAGS>::KS, DB = Wave<D, NW, F16, FLAGS>::DB;
   constexpr int NQK = 2 * KS;  // score slots
   constexpr int NPV = 4 * DB;  // P V slots, half of them per 32 keys
-  const uint8_t *ks_ = smem + w.k_slot(PAR ^ 1) * TL::kBytes;
-  const uint8_t *vs_ = smem + w.v_slot(PAR) * TL::kBytes;
+  const uint8_t *ks_ = smem + (PAR ^ 1) * TL::kBytes;
+  const uint8_t *vs_ = smem + (2 + PAR) * TL::kBytes;
   // Score fragment f: key half kb = f & 1, k-step ks = f >> 1.
   auto k_frag = [&](int f) -> u32x4 {
     return *reinterpret_cast<const u32x4 *>(ks_ + w.k_read[f >> 1] + (f & 1) * 32 * TL::kRowBytes);
@@ -638,7 +632,7 @@ __device__ __forceinline__ void hot_step(Wave<D, NW, F16, FLAGS> &w, const uint8
     bm = __builtin_fmaxf(p.a, p.b);
   }
   w.l_run = w.l_run * corr + ((bs[0] + bs[1]) + (bs[2] + bs[3]));
-  if constexpr ((FLAGS & kStaged) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, PAR);
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, PAR);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
   __syncthreads();
 }
@@ -662,7 +656,7 @@ __device__ __forceinline__ void edge_step(Wave<D, NW, F16, FLAGS> &w, const uint
   float corr;
   const float m_exp = adopt_maximum<D, NW>(w, bm, corr);
 
-  const uint8_t *vs_ = smem + w.v_slot(par) * TL::kBytes;
+  const uint8_t *vs_ = smem + (2 + par) * TL::kBytes;
   float bs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   uint32_t pk[16];
   if constexpr (D > 64) {  // both halves always, in one piece for the scheduler
@@ -685,7 +679,7 @@ __device__ __forceinline__ void edge_step(Wave<D, NW, F16, FLAGS> &w, const uint
     seen = halves_seen<D, NW, CAUSAL>(w, blk + 1, kbits_next);
     bm = -INFINITY;
     if (D > 64 || !w.ranged || seen != 0) {
-      scores<D, NW>(w, smem, w.k_slot(par ^ 1), sv);
+      scores<D, NW>(w, smem, par ^ 1, sv);
       if (!w.positive) {
 #pragma unroll
         for (int i = 0; i < 32; i++) sv[i] *= w.c_exp;
@@ -695,7 +689,7 @@ __device__ __forceinline__ void edge_step(Wave<D, NW, F16, FLAGS> &w, const uint
       bm = row_max(sv);
     }
   }
-  if constexpr ((FLAGS & kStaged) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, par);
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, par);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
   __syncthreads();
 }
@@ -706,7 +700,7 @@ __device__ __forceinline__ void idle_step(Wave<D, NW, F16, FLAGS> &w, uint8_t *s
   const int par = blk & 1;
   fill_v<D, NW>(w, blk + 1, par ^ 1);
   fill_k<D, NW>(w, blk + 2, par);
-  if constexpr ((FLAGS & kStaged) != 0) land_pages<D, NW>(w, smem, blk, par);
+  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, smem, blk, par);
   __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 }

@@ -235,13 +235,12 @@ struct PagedArgs {
 };
 // The most query heads a KV head serves: a tile holds whole tokens.
 constexpr int32_t kMostPagedGroup = 128;
-// A call's form: query rows of a tile, 32 or 128.
+// A call's form: query rows of a tile, 16, 32 or 128.
 int paged_tile_rows(const PagedArgs &a);
-// The most partial states a call can leave, and the size of one.
+// The most partial states a call can leave, and the bytes for them.
 int64_t paged_slots(const PagedArgs &a);
-int64_t paged_slot_floats(const PagedArgs &a);
-int64_t paged_workgroups(const PagedArgs &a);
 int64_t paged_workspace(const PagedArgs &a);
+int64_t paged_workgroups(const PagedArgs &a);
 hipError_t launch_paged(const PagedArgs &a, hipStream_t stream);
 const char *paged_config(const PagedArgs &a);
 // One head size's kernels each.

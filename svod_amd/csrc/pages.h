@@ -50,19 +50,6 @@ __device__ __forceinline__ int64_t page_row(const PagesArgs &p, int page, int he
   return ((int64_t)page * p.kv_heads + head) << p.page_log2;
 }
 
-// x summed over the lanes up to and with this one.
-__device__ __forceinline__ int sum_to_lane(int x) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-#endif
-  return x;
-}
-
 // 2^e for a scale's byte e + 127.  (The writer's bytes are 10 to 247: never the two that are no power of two in f32.)
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 

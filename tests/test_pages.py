@@ -91,9 +91,9 @@ def test_the_workspace_follows_the_form():
     assert w(Q, long, Attn(causal=True, splits=1)) == 0
     few, many = w(Q, long, Attn(causal=True)), w(t(900, 4, 64), long, Attn(causal=True))
     state = lambda rows: rows * 66 * 4
-    assert (few - 16) % state(32) == 0 and (many - 16) % state(128) == 0
+    assert (few - 16) % state(16) == 0 and (many - 16) % state(128) == 0
     # Five rows of three sequences: a tile each, of two KV heads.
-    assert w(Q, long, Attn(causal=True, splits=7)) == 3 * 2 * 7 * state(32) + 16
+    assert w(Q, long, Attn(causal=True, splits=7)) == 3 * 2 * 7 * state(16) + 16
     assert w(Q, short, Attn(causal=True, splits=7)) == 0  # no more splits than key blocks: one
     # What the op would not take asks for nothing.
     assert w(t(5, 3, 64), long, Attn()) == 0 and w(Q, long, Attn(keys=KeyMask.lens(t(3, dtype=I32)))) == 0
