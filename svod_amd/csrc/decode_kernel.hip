@@ -753,20 +753,19 @@ hipError_t launch_d(const Packed &p, int rows, int mode, bool f16, hipStream_t s
   return f16 ? launch_r<D, 4, true>(p, mode, stream) : launch_r<D, 4, false>(p, mode, stream);
 }
 
-// A launch's tag: no two of a process have the same, and where they start differs from process to process.
-uint64_t next_tag() {
+std::atomic<int> g_decode_rows{kDecodeRowsDefault};
+
+}  // namespace
+
+uint64_t launch_tag() {
   static std::atomic<uint64_t> next{[] {
     uint64_t seed = 0;
     if (getrandom(&seed, sizeof seed, GRND_NONBLOCK) != (ssize_t)sizeof seed)
       seed = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15u;
     return seed;
   }()};
-  return next.fetch_add(1, std::memory_order_relaxed) & ((uint64_t)-1 >> kCountBits);
+  return next.fetch_add(1, std::memory_order_relaxed);
 }
-
-std::atomic<int> g_decode_rows{kDecodeRowsDefault};
-
-}  // namespace
 
 void attention_decode_rows(int32_t rows) {
   g_decode_rows.store(rows < 0 ? 0 : (rows > kDecodeRows ? kDecodeRows : rows), std::memory_order_relaxed);
@@ -839,7 +838,7 @@ hipError_t launch_decode(const AttnArgs &a, hipStream_t stream) {
   const bool shared = merged && a.shares && a.key_lens != nullptr && a.key_mask == nullptr && splits >= 4 &&
                       a.batch >= 4 && a.batch <= kMostSharingRows && (int64_t)a.batch * a.tk < 0x7fffffffLL &&
                       (int64_t)a.batch * a.tk * a.kv_heads * a.d * 4 >= 96 << 20;
-  if (merged) p.tag = next_tag();
+  if (merged) p.tag = launch_tag() & ((uint64_t)-1 >> kCountBits);
   const int mode = splits == 1 ? kWhole : !merged ? kPartial : shared ? kShared : kMerged;
   switch (a.d) {
     case 32: return launch_d<32>(p, rows, mode, a.f16 != 0, stream);

@@ -171,6 +171,8 @@ bool attention_decodes(const AttnArgs &a, int32_t limit);
 void attention_decode_rows(int32_t rows);
 int32_t attention_decode_limit();
 hipError_t launch_decode(const AttnArgs &a, hipStream_t stream);
+// A launch's tag: no two of a process have the same, and where they start differs from process to process.
+uint64_t launch_tag();
 // The most KV heads (log2) a workgroup of the decoder step's kernel takes: as many as make 512 bytes of a key row, four at
 // most, where they divide the heads.
 constexpr int decode_most_heads(int32_t d, uint32_t kv_heads) {

@@ -1,9 +1,10 @@
 // What the kernels of attention over pages share: a launch's parameters, the deal of its work, and the pages of a wave's keys.
 //
-// How many tokens each sequence has is device data.  Every wave works the launch's deal out for itself, a lane a sequence: the
-// tiles and key blocks of all sequences give the blocks an item may have, a tile of more blocks is split, items are numbered
-// sequence by sequence, a tile's splits next to each other, and a workgroup finds its item from sums over the lanes.  The host
-// knows bounds only (paged_workgroups), and workgroups past the last item leave at once.
+// How many tokens each sequence has is device data.  Every wave works the launch's deal out for itself, a lane a sequence.  A
+// tile of query rows has parts: one, or as many as make its parts short enough to keep the chip busy, or one a key block.  The
+// parts of a KV head are numbered sequence by sequence, a tile's next to each other, and a workgroup takes a run of them: one part, or, of
+// parts of a block, an even share of all.  So it finds its own from sums over the lanes.  The host knows bounds only
+// (paged_workgroups), and workgroups past the last part leave at once.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -45,7 +46,9 @@ struct PagedParams {
   const void *k, *v, *k_scale, *v_scale;
   const int32_t *table;
   float *parts;
-  int32_t *told;  // behind them: the blocks an item had
+  int32_t *told;        // behind them: the deal, for the merge of tiles of 128 rows
+  uint64_t *arrivals;   // or a word a workgroup, for those of few rows, of any content
+  uint64_t tag;         // the launch's
   int32_t columns, pages, page_log2;
   int32_t heads, group;
   uint32_t group_rcp;
@@ -53,6 +56,7 @@ struct PagedParams {
   float scale;
   int32_t splits;        // as in PagedArgs
   int32_t slots;         // partial states there is room for
+  int32_t shares;        // whether workgroups may take shares of all blocks: few rows, and tiles for more than half of the chip's places
   // Of blocks_an_item(): the fewest blocks of an item, the workgroups that the chip holds at a time; and in us a block of a
   // workgroup by itself and with company on its compute unit, a state of every row, and a block's bytes at the rate that memory gives.
   float least;
@@ -73,6 +77,14 @@ __device__ __forceinline__ uint32_t over(uint32_t n, uint32_t d, uint32_t rcp) {
 }
 __device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 __device__ __forceinline__ int lane_id() { return (int)__builtin_amdgcn_workitem_id_x() & 63; }
+// The same, of which the compiler knows nothing: what a turn works out from it is not kept in registers from one to the next.
+__device__ __forceinline__ int lane_of_turn() {
+  int lane = lane_id();
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(lane));
+#endif
+  return lane;
+}
 
 // x folded over the lanes up to and with this one, with `op` of a lane's value and the one before it; op(0, x) is x.
 template <typename T, typename Op>
@@ -93,7 +105,7 @@ __device__ __forceinline__ int sum_to(int x) {
   return fold_to_lane(x, [](int a, int b) { return a + b; });
 }
 
-constexpr float kMerge = 5.0f;  // us, the merge's launch
+constexpr float kStart = 5.0f, kMerge = 5.0f;  // us: from a part's place to its first block, and the merge
 // What a lane's sequence asks for: tiles of query rows, and the key blocks of one of its tiles at most.
 struct Demand {
   int start, fresh, len;  // as in Sequence
@@ -119,119 +131,179 @@ __device__ __forceinline__ Demand demand_of(const Deal &d, int b) {
   return x;
 }
 
-constexpr int kNoSplits = 0x7fffffff;  // an item's blocks where none is split
-// A tile's splits where an item has `most` blocks.  (The estimate is off by one at most: there are no more splits than places.)
-__device__ __forceinline__ int splits_of(const PagedParams &p, int blocks, int most) {
+constexpr int kNoSplits = 0x7fffffff;  // a part's blocks where no tile is split
+// The blocks that a part of a split tile has at most, and the parts that a workgroup takes: more than one are of a block each.
+struct Parts {
+  int most, run;
+};
+// A tile's parts.  (The estimate is off by one at most: there are no more parts than places.)
+__device__ __forceinline__ int parts_of(const PagedParams &p, int blocks, const Parts &parts) {
   if (p.splits != 0) return max(1, min(p.splits, blocks));
-  if (most == kNoSplits) return 1;
-  const int up = blocks + most - 1;
-  int n = (int)((float)up * __builtin_amdgcn_rcpf((float)most));
-  n -= n * most > up ? 1 : 0;
-  n += up - n * most >= most ? 1 : 0;
+  if (parts.run > 1) return max(blocks, 1);
+  if (parts.most == kNoSplits) return 1;
+  const int up = blocks + parts.most - 1;
+  int n = (int)((float)up * __builtin_amdgcn_rcpf((float)parts.most));
+  n -= n * parts.most > up ? 1 : 0;
+  n += up - n * parts.most >= parts.most ? 1 : 0;
   return max(n, 1);
 }
-// The key blocks an item may have.  W blocks of all tiles in items of n are W / n + tiles items at most.  With a tile for half
-// of the chip's places or fewer, n is what keeps all items on places at once (a few more than there are places would wait for a
-// whole round); with more, n makes two items a place, which then even out.  Splitting has to win back its merge and
-// the states that it writes and reads: it does not for tiles that are short, nor for ones that are alike and many.
+// W blocks of all tiles in parts of n are W / n + tiles parts at most.  With a tile for half of the chip's places or fewer, n is what
+// keeps all parts on places at once (a few more than there are places would wait for a whole round).  With more tiles
+// they are whole, but: where rows are few and the lengths differ so much or leave a last round so empty that it pays, every place
+// takes an even share of all blocks, in which a few tiles begin and end; of tiles of 128 rows, which want their sequence's
+// others beside them in the same L2 (4 chunks of 2048 over 16384 keys 964 us, 1072 in shares), only those are split that are more than
+// twice what a place has of all blocks.  Splitting has to win back its merge and the states that it writes and reads, a
+// share the start of every tile in it.
 // This stands in front of a workgroup's first load, and what it costs is its length: a launch's instructions come from memory the
-// first time.  (Five counts of items weighed against each other, by sums over the lanes each, were 1.3 us where this is XX.)
-__device__ __forceinline__ int blocks_an_item(const Deal &deal, const PagedParams &p, const Demand &first) {
-  if (p.splits != 0) return kNoSplits;
+// first time.  (Five counts of parts weighed against each other, by sums over the lanes each, were 1.3 us where this is 0.5.)
+template <bool SHARES>
+__device__ __forceinline__ Parts parts_of_all(const Deal &deal, const PagedParams &p, const Demand &first) {
+  Parts parts = {kNoSplits, 1};
+  if (p.splits != 0) return parts;
   const int lane = lane_id();
-  float work = 0.0f;
-  int longest = 0, tiles = 0;
+  int work = 0, longest = 0, tiles = 0;
   for (int base = 0; base < deal.batch; base += 64) {
     const Demand d = base == 0 ? first : demand_of(deal, base + lane);
-    work += (float)d.tiles * (float)d.blocks;
+    work += d.tiles * max(d.blocks, 1);
     longest = max(longest, d.tiles > 0 ? d.blocks : 0);
     tiles += d.tiles;
   }
-  const float heads = (float)deal.kv_heads, places = (float)p.places;
-  const float blocks = heads * __uint_as_float((uint32_t)last_lane((int)__float_as_uint(fold_to_lane(work, [](float a, float b) { return a + b; }))));
-  const float units = heads * (float)last_lane(sum_to(tiles)), most = (float)last_lane(fold_to_lane(longest, [](int a, int b) { return max(a, b); }));
-  const bool sparse = units * 2.0f <= places;
-  const float n = __builtin_fmaxf(p.least, __builtin_ceilf(blocks * __builtin_amdgcn_rcpf(sparse ? places - units : 2.0f * places) * (1.0f + 1e-6f)));
-  // In us: a tile whole, or its items one after the other, as many rounds as there are; and what memory takes.
-  const float stream = blocks * p.stream;
-  const float whole = __builtin_fmaxf(most * (sparse ? p.step : p.crowded), stream);
-  const float split = __builtin_fmaxf(sparse ? n * p.crowded : blocks * __builtin_amdgcn_rcpf(places) * p.crowded + 0.5f * n * p.crowded, stream) +
-                      kMerge + p.states * (blocks * __builtin_amdgcn_rcpf(n * units) + 1.0f);
-  return n < most && split < whole ? (int)n : kNoSplits;
+  const int blocks = last_lane(sum_to(work));  // of a KV head's tiles
+  const float heads = (float)deal.kv_heads, places = (float)p.places, a_place = __builtin_amdgcn_rcpf(places);
+  const float all = heads * (float)blocks, units = heads * (float)last_lane(sum_to(tiles));
+  const float most = (float)last_lane(fold_to_lane(longest, [](int a, int b) { return max(a, b); }));
+  const float stream = all * p.stream;
+  if (units * 2.0f <= places) {
+    const float n = __builtin_fmaxf(p.least, __builtin_ceilf(all * __builtin_amdgcn_rcpf(places - units) * (1.0f + 1e-6f)));
+    const float whole = __builtin_fmaxf(most * p.step, stream);
+    const float split = __builtin_fmaxf(n * p.crowded, stream) + kMerge + p.states * (all * __builtin_amdgcn_rcpf(n * units) + 1.0f);
+    if (n < most && split < whole) parts.most = (int)n;
+  } else if (!SHARES) {
+    const float n = __builtin_fmaxf(p.least, __builtin_ceilf(2.0f * all * a_place * (1.0f + 1e-6f)));
+    const float rest = all * a_place * p.crowded;
+    if (p.slots > 0 && n < most && rest + 0.5f * n * p.crowded + kMerge + p.states * (all * __builtin_amdgcn_rcpf(n * units) + 1.0f) < most * p.step)
+      parts.most = (int)n;
+  } else if constexpr (SHARES) {
+    const int share = p.places / deal.kv_heads > 0 ? (blocks + p.places / deal.kv_heads - 1) / (p.places / deal.kv_heads) : blocks;
+    const float rounds = __builtin_ceilf(units * a_place);
+    const float whole = __builtin_fmaxf(most, rounds * all * __builtin_amdgcn_rcpf(units)) * p.crowded;
+    const float shared = all * a_place * p.crowded + kStart * units * a_place + kMerge + p.states;
+    if (p.slots > 0 && share > 1 && shared < whole) parts.run = share;
+  }
+  return parts;
 }
 
-// Where an item, or a row, is in the deal.
+// Where a part of a KV head, or a packed row, is in the deal.
 struct Place {
-  int b, tile, split, splits;
-  int slot;  // of the tile's first split, in KV heads' states
+  int b, tile;
+  int part, parts;   // of the tile's
+  int tile_at;       // the number of its first part
   Sequence s;
   bool found;
 };
-// The item-th item; or, with BY_ROW, the tile of packed row `item`.
+// The part of number `at`; or, with BY_ROW, the tile of packed row `at`.
 template <bool BY_ROW>
-__device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p, int item, const Demand &first, int most) {
+__device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p, int at, const Demand &first, const Parts &all) {
   const int lane = lane_id();
-  const bool splitting = p.splits > 1 || most != kNoSplits;
-  Place at{};
-  int items_before = 0, slots_before = 0;
+  Place x{};
+  int before = 0;
   for (int base = 0; base < deal.batch; base += 64) {
     const Demand d = base == 0 ? first : demand_of(deal, base + lane);
-    const int splits = splitting ? splits_of(p, d.blocks, most) : 1, items = d.tiles * splits;
-    const int items_to = BY_ROW ? 0 : sum_to(items);
-    const uint64_t here = BY_ROW ? __builtin_amdgcn_ballot_w64(d.start <= item && item - d.start < d.fresh)
-                                 : __builtin_amdgcn_ballot_w64(items_to > item - items_before);
-    const int slots = splits > 1 ? items : 0, slots_to = splitting ? sum_to(slots) : 0;
+    const int parts = parts_of(p, d.blocks, all), sum = d.tiles * parts, to = sum_to(sum);
+    const uint64_t here = BY_ROW ? __builtin_amdgcn_ballot_w64(d.start <= at && at - d.start < d.fresh)
+                                 : __builtin_amdgcn_ballot_w64(to > at - before);
     if (here != 0) {
       const int at_lane = __builtin_ctzll(here);
-      at.b = base + at_lane;
-      at.splits = __builtin_amdgcn_readlane(splits, at_lane);
-      at.s.start = __builtin_amdgcn_readlane(d.start, at_lane);
-      at.s.fresh = __builtin_amdgcn_readlane(d.fresh, at_lane);
-      at.s.len = __builtin_amdgcn_readlane(d.len, at_lane);
-      const int tiles = __builtin_amdgcn_readlane(d.tiles, at_lane);
+      x.b = base + at_lane;
+      x.parts = __builtin_amdgcn_readlane(parts, at_lane);
+      x.s.start = __builtin_amdgcn_readlane(d.start, at_lane);
+      x.s.fresh = __builtin_amdgcn_readlane(d.fresh, at_lane);
+      x.s.len = __builtin_amdgcn_readlane(d.len, at_lane);
+      const int tiles = __builtin_amdgcn_readlane(d.tiles, at_lane), start = before + __builtin_amdgcn_readlane(to - sum, at_lane);
       int order;  // the last tile, which sees the most keys, comes first
       if (BY_ROW) {
-        at.tile = (int)over((uint32_t)(item - at.s.start), (uint32_t)deal.tokens, deal.tokens_rcp);
-        order = tiles - 1 - at.tile;
+        x.tile = (int)over((uint32_t)(at - x.s.start), (uint32_t)deal.tokens, deal.tokens_rcp);
+        order = tiles - 1 - x.tile;
       } else {
-        const int within = item - items_before - __builtin_amdgcn_readlane(items_to - items, at_lane);
-        order = at.splits == 1 ? within : within / at.splits;
-        at.split = within - order * at.splits;
-        at.tile = tiles - 1 - order;
+        const int within = at - start;
+        order = x.parts == 1 ? within : (int)((uint32_t)within / (uint32_t)x.parts);
+        x.part = within - order * x.parts;
+        x.tile = tiles - 1 - order;
       }
-      at.slot = slots_before + __builtin_amdgcn_readlane(slots_to - slots, at_lane) + order * at.splits;
-      at.found = true;
-      return at;
+      x.tile_at = start + order * x.parts;
+      x.found = true;
+      return x;
     }
-    items_before += last_lane(items_to);
-    slots_before += last_lane(slots_to);
+    before += last_lane(to);
   }
-  return at;
+  return x;
 }
 
-// A workgroup's item: the KV heads of one are neighbours in the launch, their pages are neighbours in memory.
+// What a workgroup does: parts [at, to) of a KV head.  The KV heads of a part are neighbours in the launch, their pages are
+// neighbours in memory.
+struct Turn {
+  int kvh, mine, at, to;
+  Parts parts;
+  Demand first;
+};
+template <bool SHARES>
+__device__ __forceinline__ Turn turn_of(const Deal &deal, const PagedParams &p) {
+  const uint32_t wg = __builtin_amdgcn_workgroup_id_x();
+  Turn t;
+  t.mine = (int)over(wg, (uint32_t)deal.kv_heads, deal.kvh_rcp);
+  t.kvh = (int)(wg - (uint32_t)t.mine * (uint32_t)deal.kv_heads);
+  t.first = demand_of(deal, lane_id());
+  t.parts = parts_of_all<SHARES>(deal, p, t.first);
+  t.at = t.mine * t.parts.run;
+  t.to = t.at + t.parts.run;
+  // The merge's kernel goes by the same deal: it is told what this launch went by.
+  if (p.told != nullptr && wg == 0 && __builtin_amdgcn_workitem_id_x() == 0) p.told[0] = t.parts.most, p.told[1] = t.parts.run;
+  return t;
+}
+// The workgroups that have a tile of several parts: one a part, or those in whose shares it lies; and the slots of their partial
+// states, one a workgroup, or two where they take shares, of the tile that a share begins in and of the one that it ends in.
+struct Sharers {
+  int first, last;    // workgroups of the KV head
+  int64_t slot, next; // the first one's, and the second one's
+  int step;           // from there on
+};
+__device__ __forceinline__ Sharers sharers_of(const Deal &deal, const Place &at, int kvh, const Parts &parts) {
+  Sharers x;
+  x.first = parts.run > 1 ? at.tile_at / parts.run : at.tile_at;
+  x.last = parts.run > 1 ? (at.tile_at + at.parts - 1) / parts.run : at.tile_at + at.parts - 1;
+  const int each = parts.run > 1 ? 2 : 1;
+  x.slot = ((int64_t)x.first * deal.kv_heads + kvh) * each + (at.tile_at != x.first * parts.run ? 1 : 0);
+  x.next = ((int64_t)(x.first + 1) * deal.kv_heads + kvh) * each;
+  x.step = deal.kv_heads * each;
+  return x;
+}
+// A tile's parts from the first of a turn's on, as many as the turn has left of them.
 struct Work {
   Place at;
   int kvh;
-  int slot;  // where its partial state goes, of a split tile
-  int first, end;            // its key blocks
-  int tile_first, last;      // the tile's first token, and its last, of the sequence's new ones
+  int taken;             // of the tile's parts
+  bool whole;
+  Sharers sharers;       // of a tile that is not whole
+  int64_t slot;          // and where its partial state goes
   bool some;
+  int first, end;        // its key blocks
+  int tile_first, last;  // the tile's first token, and its last, of the sequence's new ones
 };
-__device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p) {
-  const uint32_t wg = __builtin_amdgcn_workgroup_id_x();
+template <bool SHARES>
+__device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p, const Turn &t) {
   Work w{};
-  const int item = (int)over(wg, (uint32_t)deal.kv_heads, deal.kvh_rcp);
-  w.kvh = (int)(wg - (uint32_t)item * (uint32_t)deal.kv_heads);
-  const Demand first_demand = demand_of(deal, lane_id());
-  const int most = blocks_an_item(deal, p, first_demand);
-  w.at = place_of<false>(deal, p, item, first_demand, most);
-  // The merge goes by the same deal: it is told what this launch went by, behind the states.
-  if (wg == 0 && __builtin_amdgcn_workitem_id_x() == 0 && p.slots > 0) *p.told = most;
-  w.slot = (w.at.slot + w.at.split) * deal.kv_heads + w.kvh;
-  // (Slots there is no room for: starts that descend give more rows than there are.)
-  w.some = w.at.found && (w.at.splits == 1 || w.slot < p.slots);
-  if (!w.some) return w;
+  w.kvh = t.kvh;
+  w.at = place_of<false>(deal, p, t.at, t.first, t.parts);
+  if (!w.at.found) return w;
+  w.taken = SHARES ? min(w.at.parts - w.at.part, t.to - t.at) : 1;
+  w.whole = w.taken == w.at.parts;
+  w.some = true;
+  if (!w.whole) {
+    w.sharers = sharers_of(deal, w.at, t.kvh, t.parts);
+    const int which = t.mine - w.sharers.first;
+    w.slot = which == 0 ? w.sharers.slot : w.sharers.next + (int64_t)(which - 1) * w.sharers.step;
+    w.some = w.slot < p.slots;  // (there is no room: starts that descend give more rows than there are)
+  }
   const Sequence &s = w.at.s;
   w.tile_first = w.at.tile * deal.tokens;
   w.last = min(w.tile_first + deal.tokens, s.fresh) - 1;
@@ -243,11 +315,18 @@ __device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p) 
   }
   first = min(first / kKeys, (end + kKeys - 1) / kKeys);
   end = (end + kKeys - 1) / kKeys;
-  if (w.at.splits > 1) {
-    // An even share of the tile's blocks, the first splits' one more where they do not go up.
-    const int n = end - first, each = n / w.at.splits, more = n - each * w.at.splits;
-    first += w.at.split * each + min(w.at.split, more);
-    end = first + each + (w.at.split < more ? 1 : 0);
+  if (!w.whole) {
+    const int n = end - first;
+    if (SHARES && t.parts.run > 1) {
+      // A part a block, of as many as the sequence's longest tile has.
+      end = first + min(n, w.at.part + w.taken);
+      first += min(n, w.at.part);
+    } else {
+      // An even share of the tile's blocks, the first parts' one more where they do not go up.
+      const int each = n / w.at.parts, more = n - each * w.at.parts;
+      first += w.at.part * each + min(w.at.part, more);
+      end = first + each + (w.at.part < more ? 1 : 0);
+    }
   }
   w.first = uniform(first);
   w.end = uniform(end);
@@ -313,6 +392,9 @@ struct PagedLaunch {
 };
 PagedLaunch paged_launch(const PagedArgs &a);
 constexpr int kPagedUnits = 256;  // compute units of an MI355X
+// A word of arrivals: its low bits count, the others are the launch's tag.  Words are on lines of their own.
+constexpr int kPagedCountBits = 20, kPagedWord = 16;
+constexpr uint64_t kPagedEnded = (1 << kPagedCountBits) - 1, kPagedTags = (uint64_t)-1 >> kPagedCountBits;
 // The form of few rows (paged_few_kernel.hip), and its workgroups that a compute unit holds at a time.
 hipError_t launch_paged_few(const PagedArgs &a, const PagedLaunch &l, hipStream_t stream);
 int paged_few_resident(int d, int rows);

@@ -12,7 +12,8 @@
 //     into a tile of the wave's own, codes widened on the way.  No wave waits for another inside the loop.
 //   - the four waves of a workgroup take an item's key blocks in turn, each with its own state; K of a wave's next block is asked
 //     for when its scores are done, V when the tile is written: 32 KiB in flight a wave at D 128, 8 waves a compute unit.
-//   - their states meet in LDS at the end, the item's in merge_kernel.
+//   - their states meet in LDS at the end; those of the workgroups that share a tile in memory, where the one that counts itself in
+//     last adds them up.
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"
@@ -47,10 +48,12 @@ struct Few {
   static constexpr int kStateRow = (D + 4) * 4;
   static constexpr int kState = kRows * kStateRow + kRows * 8;
   static constexpr int kWaveLds = kTile > kState ? kTile : kState;
-  static constexpr int kLds = kWaves * kWaveLds;
+  static constexpr int kLds = kWaves * kWaveLds;  // and a word behind
+  // A state in memory: the rows' columns, then their maxima and sums.
+  static constexpr int kStateBytes = kRows * (D + 2) * 4;
   // Waves a SIMD, which are workgroups a compute unit: by registers and LDS.
   static constexpr int kResident = D == 256 || (D == 128 && RT == 2) ? 1 : (D == 128 || RT == 2) ? 2 : 3;
-  static_assert(kResident * kLds <= 160 * 1024, "the workgroups' LDS");
+  static_assert(kResident * (kLds + 16) <= 160 * 1024, "the workgroups' LDS");
 };
 // A tile of V is read by 16 lanes as 4 rows of 32 bytes, 8 rows to half a wave: the 32-byte groups of a row are xor-ed with what
 // tells 8 rows apart within the period of the banks (256 bytes: a row of 128 values, half of one of 256, two of 64).
@@ -73,6 +76,42 @@ __device__ __forceinline__ float over_quarters(float x, Op op) {
   return x;
 }
 
+// Partial states that another workgroup reads go past the L2s, each of which serves one XCD, and are read the same way: stores and
+// loads that are coherent over the device (the instructions' sc1 bit).
+struct States {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __amdgpu_buffer_rsrc_t rsrc;
+  static constexpr int kDevice = 16;
+  __device__ __forceinline__ States(float *p, uint32_t bytes) : rsrc(__builtin_amdgcn_make_buffer_rsrc(p, 0, (int)bytes, 0x00020000)) {}
+  __device__ __forceinline__ void put4(uint32_t at, const f32x4 &x) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rsrc, (int)at, 0, kDevice);
+  }
+  __device__ __forceinline__ void put2(uint32_t at, const f32x2 &x) const {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), rsrc, (int)at, 0, kDevice);
+  }
+  __device__ __forceinline__ f32x4 got4(uint32_t at) const {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, 0, kDevice));
+  }
+  __device__ __forceinline__ f32x2 got2(uint32_t at) const {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)at, 0, kDevice));
+  }
+#endif
+};
+// A row's state over some of its keys, eight columns of it, the maximum in the exponent's units; and another's joined to it.
+struct State {
+  float m, l, o[8];
+  __device__ __forceinline__ void join(float m2, float l2, const f32x4 &a, const f32x4 &b, bool there = true) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float top = __builtin_fmaxf(m, m2), mine = __builtin_amdgcn_exp2f(m - top);
+    const float weight = there ? __builtin_amdgcn_exp2f(m2 - top) : 0.0f;
+    m = top;
+    l = l * mine + l2 * weight;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = o[i] * mine + (i < 4 ? a[i % 4] : b[i % 4]) * weight;
+#endif
+  }
+};
+
 template <int D, int RT, bool F16, bool CODED>
 __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const PagedParams &p, const Work &work) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -82,7 +121,7 @@ __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const 
   constexpr int KL = kRowBytes / 64;            // loads of 16 keys' rows
   constexpr int DB = D / 16;                    // column blocks of O
   constexpr int kVLanes = kRowBytes / 16, kVRows = 64 / kVLanes, kVPer = 16 / kVRows;  // V: lanes a row, rows a load, loads a run of 16 rows
-  const int lane = lane_id(), wave = uniform((int)__builtin_amdgcn_workitem_id_x() >> 6);
+  const int lane = lane_of_turn(), wave = uniform((int)__builtin_amdgcn_workitem_id_x() >> 6);
   const int lr = lane & 15, lq = lane >> 4;
 
   const int first_key = work.first * kKeys, end = work.end - work.first;  // the item's own frame: keys count from its first
@@ -158,6 +197,16 @@ __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const 
       }
     }
   };
+  // The word in which the workgroups of a tile count themselves in is the workspace's and holds anything at first.  Every one
+  // makes sure, before it counts, that it carries this launch's tag: it becomes (tag, 0) by one compare-and-swap out of whatever was
+  // there, and no other write of the launch leaves that content again, so a late swap out of it fails.  Nothing else ever carries
+  // the tag but the word as an earlier replay of the same captured launch left it, and that one counts kPagedEnded, which
+  // no word of a launch under way does.  The content is asked for ahead of the keys, the swap goes out behind the loop: neither is
+  // waited for.
+  uint64_t *const word = work.whole ? nullptr : p.arrivals + ((int64_t)work.sharers.first * deal.kv_heads + work.kvh) * kPagedWord;
+  const bool counts = !work.whole && wave == 0 && lane == 0;
+  uint64_t found = 0;
+  if (counts) found = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   find(wave);
   ask_k();
   ask_v();
@@ -291,6 +340,8 @@ __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const 
     }
   }
 
+  if (counts && (found >> kPagedCountBits != p.tag || (found & kPagedEnded) == kPagedEnded))
+    __hip_atomic_compare_exchange_strong(word, &found, p.tag << kPagedCountBits, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // ---- the waves' states as one: maxima in the exponent's units.
   if (L::kState > L::kTile) __syncthreads();  // a state reaches into the next wave's tile
 #pragma unroll
@@ -303,7 +354,8 @@ __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const 
   }
   __syncthreads();
   constexpr int kPieces = D / 8;  // of a row, 8 columns each
-  for (int c = (int)__builtin_amdgcn_workitem_id_x(); c < L::kRows * kPieces; c += kWaves * 64) {
+  const States states(p.parts, (uint32_t)p.slots * L::kStateBytes);
+  for (int c = wave * 64 + lane; c < L::kRows * kPieces; c += kWaves * 64) {
     const int row = c / kPieces, column = c % kPieces * 8;
     const Row r = row_of_tile(deal, p, work, row);
     f32x2 ml[kWaves];
@@ -327,37 +379,112 @@ __device__ __forceinline__ void few_item(uint8_t *smem, const Deal &deal, const 
       for (int i = 0; i < 8; i++) o[i] += x[w][i / 4][i % 4] * weight;
     }
     if (!r.there) continue;
-    if (work.at.splits > 1) {
-      float *part = p.parts + (int64_t)work.slot * (L::kRows * (D + 2));
-      if (column == 0) part[L::kRows * D + row] = top, part[L::kRows * (D + 1) + row] = sum;
-      float *to = part + row * D + column;
-      *reinterpret_cast<f32x4 *>(to) = f32x4{o[0], o[1], o[2], o[3]};
-      *reinterpret_cast<f32x4 *>(to + 4) = f32x4{o[4], o[5], o[6], o[7]};
-    } else {
+    if (work.whole) {
       const float inv = 1.0f / (sum == 0.0f ? 1.0f : sum);
       u32x4 out;
 #pragma unroll
       for (int i = 0; i < 4; i++) out[i] = narrow<F16>(o[2 * i] * inv, o[2 * i + 1] * inv);
       *reinterpret_cast<u32x4 *>(p.o + r.at * D + column) = out;
+    } else {
+      const uint32_t at = (uint32_t)work.slot * L::kStateBytes;
+      if (column == 0) states.put2(at + (L::kRows * D + 2 * row) * 4, f32x2{top, sum});
+      states.put4(at + (row * D + column) * 4, f32x4{o[0], o[1], o[2], o[3]});
+      states.put4(at + (row * D + column + 4) * 4, f32x4{o[4], o[5], o[6], o[7]});
     }
+  }
+  if (work.whole) return;
+
+  // ---- the tile's other workgroups.  This one's state is where every other sees it before it counts itself in: it was stored
+  // past the L2s, and vmcnt is at zero when the memory behind those has taken it.  No one waits for anyone.
+  const int others = work.sharers.last - work.sharers.first;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int *const arrived = reinterpret_cast<int *>(smem + L::kLds);
+  if (counts) {
+    const uint64_t before = __hip_atomic_fetch_add(word, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = (int)(before & kPagedEnded) == others;
+    if (last) __hip_atomic_store(word, p.tag << kPagedCountBits | kPagedEnded, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *arrived = last ? 1 : 0;
+  }
+  __syncthreads();
+  if (uniform(*arrived) == 0) return;
+  asm volatile("" ::: "memory");  // the states are read from here on
+  // The last one has 256 threads for rows * kPieces pieces: where they are fewer, several take a piece's states in turn and join theirs
+  // in LDS.  Who adds what follows from the sizes alone: the same bits whoever is last.
+  const int rows = (work.last - work.tile_first + 1) * p.group, pieces = rows * kPieces;
+  int teams_log2 = 0;
+  while (pieces << (teams_log2 + 1) <= kWaves * 64 && (1 << teams_log2) <= others) teams_log2++;
+  const int id = wave * 64 + lane, team = id / pieces, teams = 1 << teams_log2;
+  constexpr int kAhead = 4;
+  for (int c = teams > 1 ? id - team * pieces : id; c < pieces; c += teams > 1 ? pieces : kWaves * 64) {
+    const int row = c / kPieces, column = c % kPieces * 8;
+    State x{kNone, 0.0f, {}};
+    if (team < teams || teams == 1) {
+      const int from = teams > 1 ? team : 0;
+      for (int i = from; i <= others; i += teams * kAhead) {
+        f32x2 ml[kAhead];
+        f32x4 o[kAhead][2];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {  // one past the last asks for the last again, and weighs nothing
+          const int which = min(i + j * teams, others);
+          const int64_t slot = which == 0 ? work.sharers.slot : work.sharers.next + (int64_t)(which - 1) * work.sharers.step;
+          const uint32_t at = (uint32_t)slot * L::kStateBytes;
+          ml[j] = states.got2(at + (L::kRows * D + 2 * row) * 4);
+          o[j][0] = states.got4(at + (row * D + column) * 4);
+          o[j][1] = states.got4(at + (row * D + column + 4) * 4);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) x.join(ml[j][0], ml[j][1], o[j][0], o[j][1], i + j * teams <= others);
+      }
+    }
+    if (teams > 1) {
+      float *const joined = reinterpret_cast<float *>(smem) + id * 12;
+      if (team < teams) {
+        *reinterpret_cast<f32x4 *>(joined) = f32x4{x.m, x.l, 0.0f, 0.0f};
+        *reinterpret_cast<f32x4 *>(joined + 4) = f32x4{x.o[0], x.o[1], x.o[2], x.o[3]};
+        *reinterpret_cast<f32x4 *>(joined + 8) = f32x4{x.o[4], x.o[5], x.o[6], x.o[7]};
+      }
+      __syncthreads();
+      if (team == 0)
+        for (int t = 1; t < teams; t++) {
+          const float *from = reinterpret_cast<const float *>(smem) + (id + t * pieces) * 12;
+          x.join(from[0], from[1], *reinterpret_cast<const f32x4 *>(from + 4), *reinterpret_cast<const f32x4 *>(from + 8));
+        }
+    }
+    if (teams > 1 && team != 0) continue;
+    const Row r = row_of_tile(deal, p, work, row);
+    const float inv = 1.0f / (x.l == 0.0f ? 1.0f : x.l);
+    u32x4 out;
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = narrow<F16>(x.o[2 * i] * inv, x.o[2 * i + 1] * inv);
+    *reinterpret_cast<u32x4 *>(p.o + r.at * D + column) = out;
   }
 #endif
 }
 
-template <int D, int RT, bool F16, bool CODED>
+template <int D, int RT, bool F16, bool CODED, bool SHARES>
 __global__ __launch_bounds__(kWaves * 64, (Few<D, RT>::kResident)) void paged_few_kernel(SVODK_DEAL_PARAMS, PagedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const Deal deal = SVODK_DEAL;
-  const Work work = work_of(deal, p);
-  if (work.some) few_item<D, RT, F16, CODED>(smem, deal, p, work);
+  Turn turn = turn_of<SHARES>(deal, p);
+  do {
+    const Work work = work_of<SHARES>(deal, p, turn);
+    if (!work.at.found) return;
+    if (work.some) few_item<D, RT, F16, CODED>(smem, deal, p, work);
+    if (SHARES) __syncthreads();  // the states have been read
+    turn.at += work.taken;
+    if (SHARES) turn.first = demand_of(deal, lane_of_turn());  // asked for again: held in registers it would cost the loop five
+  } while (SHARES && turn.at < turn.to);
 #endif
 }
 
 template <int D, int RT, bool F16, bool CODED>
 hipError_t launch(const PagedLaunch &l, hipStream_t stream) {
-  constexpr int kLds = Few<D, RT>::kLds;
-  return Launch<paged_few_kernel<D, RT, F16, CODED>>::run(l.grid, kWaves * 64, kLds, kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
+  constexpr int kLds = Few<D, RT>::kLds + 16;
+  if (l.p.shares)
+    return Launch<paged_few_kernel<D, RT, F16, CODED, true>>::run(l.grid, kWaves * 64, kLds, kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
+  return Launch<paged_few_kernel<D, RT, F16, CODED, false>>::run(l.grid, kWaves * 64, kLds, kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
 }
 template <int D, int RT>
 hipError_t launch_rows(const PagedArgs &a, const PagedLaunch &l, hipStream_t stream) {

@@ -170,10 +170,9 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
   using W = Wave<D, NW, F16, kRanged | kPaged | (CODED ? kCoded : 0u)>;
   using P = decltype(W::pages);
   constexpr int BQ = NW * kWaveRows, KS = W::KS, DB = W::DB;
-  const int tid = (int)__builtin_amdgcn_workitem_id_x();
   W w;
-  w.lane = tid & 63;
-  w.wave = uniform(tid >> 6);
+  w.lane = lane_of_turn();
+  w.wave = uniform((int)__builtin_amdgcn_workitem_id_x() >> 6);
   w.g = w.lane >> 5;
   const int ln = w.lane & 31;
 
@@ -310,10 +309,10 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
 
   const Pair lp = both_halves(w.l_run);
   const float l_tot = lp.a + lp.b;
-  if (work.at.splits > 1) {
+  if (!work.whole) {
     // ---- the split's partial state: the accumulator as it stands, the maximum in the exponent's units and the sum.
     if (mine.there) {
-      float *part = p.parts + (int64_t)work.slot * (BQ * (D + 2));
+      float *part = p.parts + work.slot * (BQ * (D + 2));
       if (w.g == 0) {
         part[BQ * D + row] = w.positive ? w.m_run * w.c_exp : w.m_run;
         part[BQ * D + BQ + row] = l_tot;
@@ -354,7 +353,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void paged_kernel(SVODK_
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const Deal deal = SVODK_DEAL;
-  const Work work = work_of(deal, p);
+  const Work work = work_of<false>(deal, p, turn_of<false>(deal, p));
   if (work.some) paged_item<D, NW, F16, CODED>(smem, deal, p, work);
 #endif
 }
@@ -371,8 +370,8 @@ __global__ __launch_bounds__(256) void merge_kernel(SVODK_DEAL_PARAMS, PagedPara
   constexpr int kLanes = D / 8, kAhead = 8;
   __shared__ __attribute__((aligned(16))) f32x4 of_waves[3][64][3];
   const Deal deal = SVODK_DEAL;
-  const int most = uniform(*p.told);
-  if (most == kNoSplits && p.splits == 0) return;
+  const Parts parts = {uniform(p.told[0]), uniform(p.told[1])};
+  if (parts.most == kNoSplits && parts.run == 1 && p.splits == 0) return;
   const int lane = lane_id();
   const int wave = uniform((int)__builtin_amdgcn_workitem_id_x() >> 6);
   const Demand first_demand = demand_of(deal, lane);
@@ -381,16 +380,15 @@ __global__ __launch_bounds__(256) void merge_kernel(SVODK_DEAL_PARAMS, PagedPara
   int row = (int)(from / pieces), piece = (int)(from - (uint32_t)row * pieces), known = -1;
   Place at{};
   for (int i = 0; i < run && row < deal.rows; i++) {
-    if (row != known) at = place_of<true>(deal, p, row, first_demand, most);
+    if (row != known) at = place_of<true>(deal, p, row, first_demand, parts);
     known = row;
     const int head = piece * kMergeHeads<D> + lane / kLanes, here = min(head, p.heads - 1);
     const int kvh = (int)over((uint32_t)here, (uint32_t)p.group, p.group_rcp);
-    const int last = at.splits - 1;
-    // (Slots past the workspace's: as paged_body.  The branch is the same in all waves.)
-    if (at.found && last > 0 && (int64_t)(at.slot + last + 1) * deal.kv_heads <= p.slots) {
+    const Sharers sharers = sharers_of(deal, at, kvh, parts);
+    const int last = at.found ? sharers.last - sharers.first : 0;
+    // (Slots past the workspace's: as work_of().  The branch is the same in all waves.)
+    if (last > 0 && sharers.next + (int64_t)(last - 1) * sharers.step - kvh + deal.kv_heads <= p.slots) {
       const int in_tile = (row - at.s.start - at.tile * deal.tokens) * p.group + here - kvh * p.group;
-      const int64_t step = (int64_t)deal.kv_heads * (BQ * (D + 2));
-      const float *part = p.parts + ((int64_t)at.slot * deal.kv_heads + kvh) * (BQ * (D + 2));
       const int column = lane % kLanes * 8;
       float m = -1e30f, l = 0.0f, acc[8] = {};
       for (int base = wave * kAhead; base <= last; base += 4 * kAhead) {
@@ -398,7 +396,8 @@ __global__ __launch_bounds__(256) void merge_kernel(SVODK_DEAL_PARAMS, PagedPara
         float ms[kAhead], ls[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {  // one past the last asks for the last again, and weighs nothing
-          const float *state = part + min(base + j, last) * step;
+          const int which = min(base + j, last);
+          const float *state = p.parts + (which == 0 ? sharers.slot : sharers.next + (int64_t)(which - 1) * sharers.step) * (BQ * (D + 2));
           ms[j] = state[BQ * D + in_tile];
           ls[j] = state[BQ * D + BQ + in_tile];
           x[j][0] = *reinterpret_cast<const f32x4 *>(state + in_tile * D + column);
@@ -462,17 +461,10 @@ template <int D, bool F16, bool CODED>
 hipError_t launch(const PagedArgs &a, hipStream_t stream) {
   const int rows = paged_tile_rows(a);
   const PagedLaunch l = paged_launch(a);
-  hipError_t e;
-  if (rows == 128)
-    e = Launch<paged_kernel<D, 4, F16, CODED>>::run(l.grid, 256, Tile<D>::kLds, Tile<D>::kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
-  else
-    e = launch_paged_few(a, l, stream);
-  if (e != hipSuccess || l.p.slots == 0) return e;
-  switch (rows) {
-    case 16: return merge<D, 16, F16>(l, stream);
-    case 32: return merge<D, 32, F16>(l, stream);
-    default: return merge<D, 128, F16>(l, stream);
-  }
+  if (rows != 128) return launch_paged_few(a, l, stream);
+  const hipError_t e =
+      Launch<paged_kernel<D, 4, F16, CODED>>::run(l.grid, 256, Tile<D>::kLds, Tile<D>::kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
+  return e != hipSuccess || l.p.slots == 0 ? e : merge<D, 128, F16>(l, stream);
 }
 
 template <int D>
@@ -507,7 +499,9 @@ int resident(const PagedArgs &a) {
   return rows == 128 ? (a.pages.d <= 128 ? 2 : 1) : paged_few_resident(a.pages.d, rows);
 }
 int64_t places(const PagedArgs &a) { return (int64_t)kPagedUnits * resident(a); }
-int64_t paged_items(const PagedArgs &a);
+// Whether there may be tiles for more than half of the chip's places.
+bool dense(const PagedArgs &a) { return 2 * tiles_at_most(a) * a.pages.kv_heads > places(a); }
+int64_t blocks_at_most(const PagedArgs &a) { return (((int64_t)a.pages.columns << a.pages.page_log2) + kBkv - 1) / kBkv; }
 }  // namespace
 
 int paged_tile_rows(const PagedArgs &a) {
@@ -516,37 +510,34 @@ int paged_tile_rows(const PagedArgs &a) {
   return group <= 32 && rows <= 32ll * a.pages.batch && a.pages.d <= 128 ? 32 : 128;
 }
 
+// A state a workgroup; two where it may take a share of all blocks, which it does on the chip's places only.
 int64_t paged_slots(const PagedArgs &a) {
-  if (a.splits == 1) return 0;
-  const int64_t blocks = (((int64_t)a.pages.columns << a.pages.page_log2) + kBkv - 1) / kBkv;
-  if (a.splits > 1) return blocks > 1 ? tiles_at_most(a) * a.pages.kv_heads * a.splits : 0;
-  // A tile of b blocks is split where b > n, the blocks an item may have, into fewer than 2 b / n; W / n is at most twice the
-  // places (blocks_an_item): fewer than four a place.
-  const bool few = paged_tile_rows(a) != 128;
-  if (blocks <= (few ? 4 : 2)) return 0;
-  const int64_t all = 4ll * places(a), items = paged_items(a);
-  return all < items ? all : items;
-}
-
-// The workgroups of a launch: a split count that was named, or the most items that blocks_an_item makes, W / n + tiles with n = W /
-// (places - tiles) where tiles have half of the places or fewer, W / (2 places) else.  (Workgroups without an item cost a place the
-// deal: with one for every partial state that there might be 16 sequences over 210 to 2100 keys took 32.8 us.)
-namespace {
-int64_t paged_items(const PagedArgs &a) {
-  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, p = places(a);
+  const int64_t blocks = blocks_at_most(a), tiles = tiles_at_most(a) * a.pages.kv_heads;
+  if (a.splits == 1 || blocks <= 1) return 0;
   if (a.splits > 1) return tiles * a.splits;
-  // Fewer tiles than may be are fewer items, but for where they come under half of the places.
-  const int64_t items = 2 * tiles <= p ? p : tiles + 2 * p;
-  return (items + a.pages.kv_heads) / a.pages.kv_heads * a.pages.kv_heads;
-}
-}  // namespace
-int64_t paged_workgroups(const PagedArgs &a) {
-  return paged_slots(a) == 0 ? tiles_at_most(a) * a.pages.kv_heads : paged_items(a);
+  const bool few = paged_tile_rows(a) != 128;
+  // Too short to be worth a merge, whatever the lengths; and blocks of all tiles are counted in 31 bits.
+  if (blocks <= (few ? 8 : 4) || tiles / a.pages.kv_heads * blocks > 0x3fffffff || (dense(a) && blocks < (few ? 16 : 64))) return 0;
+  return few && dense(a) ? 2 * (places(a) + a.pages.kv_heads) : paged_workgroups(a);
 }
 
+// The workgroups of a launch: for every tile there may be, and for the chip's places where tiles may be split; for half of those more
+// where long ones alone are (parts_of_all).  (With one for every partial state that there might be 16 sequences over 210 to 2100
+// keys took 32.8 us: one without a part costs a place the deal.)
+int64_t paged_workgroups(const PagedArgs &a) {
+  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, round = a.pages.kv_heads, p = (places(a) + round) / round * round;
+  if (a.splits > 1) return tiles * a.splits;
+  if (a.splits == 1) return tiles;
+  if (dense(a) && paged_tile_rows(a) == 128) return tiles + (places(a) / 2 + round) / round * round;
+  return tiles > p ? tiles : p;
+}
+
+// The states, and behind them two words that tell the merge of tiles of 128 rows of the deal, or a word a workgroup in which those
+// that have a tile of few rows count themselves in.
+int64_t state_bytes(const PagedArgs &a) { return paged_slots(a) * paged_tile_rows(a) * (a.pages.d + 2) * 4; }
 int64_t paged_workspace(const PagedArgs &a) {
-  const int64_t slots = paged_slots(a);
-  return slots == 0 ? 0 : slots * paged_tile_rows(a) * (a.pages.d + 2) * 4 + 16;
+  const int64_t bytes = state_bytes(a);
+  return bytes == 0 ? 0 : bytes + (paged_tile_rows(a) == 128 ? 16 : paged_workgroups(a) * kPagedWord * 8);
 }
 
 PagedLaunch paged_launch(const PagedArgs &a) {
@@ -569,17 +560,27 @@ PagedLaunch paged_launch(const PagedArgs &a) {
   p.k = g.k, p.v = g.v, p.k_scale = g.k_scale, p.v_scale = g.v_scale, p.table = g.table;
   const int64_t slots = paged_slots(a);
   p.parts = a.workspace;
-  p.told = reinterpret_cast<int32_t *>(p.parts + slots * rows * (g.d + 2));
+  if (slots > 0) {
+    uint8_t *behind = reinterpret_cast<uint8_t *>(p.parts) + state_bytes(a);
+    if (few)
+      p.arrivals = reinterpret_cast<uint64_t *>(behind), p.tag = launch_tag() & kPagedTags;
+    else
+      p.told = reinterpret_cast<int32_t *>(behind);
+  }
   p.columns = g.columns, p.pages = g.pages, p.page_log2 = g.page_log2;
   p.heads = a.heads, p.group = group, p.group_rcp = rcp_of(group);
   p.causal = a.causal, p.win_left = a.win_left, p.win_right = a.win_right, p.scale = a.scale;
   p.splits = a.splits;
   p.slots = (int32_t)slots;
+  p.shares = few && slots > 0 && a.splits == 0 && dense(a);
   p.least = few ? 4.0f : 2.0f, p.places = (int32_t)places(a);
-  p.step = few ? 0.6f : 1.4f, p.crowded = few ? 0.6f : 1.75f;
-  p.states = (float)((double)g.rows * a.heads * (g.d + 2) * 8 / 5e6);          // written and read at 5 MB a us
+  p.step = few ? 0.6f : 1.4f, p.crowded = !few ? 1.75f : dense(a) ? 1.0f : 0.6f;
+  // A state is written and read at 5 MB a us: of every row, or of two tiles a place.
+  const double of_rows = (double)g.rows * a.heads, of_places = 2.0 * places(a) * rows;
+  p.states = (float)((p.shares && of_places < of_rows ? of_places : of_rows) * (g.d + 2) * 8 / 5e6);
   p.stream = few ? (float)((g.k_scale ? 128.0 : 256.0) * g.d / 6.4e6) : 0.0f;  // at 6.4 MB a us
-  l.grid = paged_workgroups(a);
+  l.grid = slots == 0 ? tiles_at_most(a) * g.kv_heads : paged_workgroups(a);
+  if (slots == 0) p.splits = 1;
   return l;
 }
 

@@ -162,6 +162,8 @@ int take_paged(const svodk_tensor *q, const svodk_pages *pages, const svodk_attn
   if (svodk::paged_slots(a) == 0) a.splits = 1;
   // A launch's workgroups are counted in 31 bits, and so are its partial states.
   if (svodk::paged_workgroups(a) > 0x7fffffff) why = SVODK_GRAPH_SHAPE;
+  // And the bytes of the states of a named count of splits in 32.
+  if (a.splits > 1 && svodk::paged_workspace(a) > 0x7fffffff) why = SVODK_GRAPH_CONFIG;
   return 0;
 }
 

@@ -87,13 +87,17 @@ def test_without_a_device_the_graph_runs(call):
 def test_the_workspace_follows_the_form():
     w = svod_amd.attention_paged_workspace
     short, long = pages(table=t(3, 4, dtype=I32)), pages(table=t(3, 400, dtype=I32))
+    state = lambda rows: rows * 66 * 4
     assert w(Q, short, Attn(causal=True)) == 0  # one key block at most: never split
     assert w(Q, long, Attn(causal=True, splits=1)) == 0
-    few, many = w(Q, long, Attn(causal=True)), w(t(900, 4, 64), long, Attn(causal=True))
-    state = lambda rows: rows * 66 * 4
-    assert (few - 16) % state(16) == 0 and (many - 16) % state(128) == 0
-    # Five rows of three sequences: a tile each, of two KV heads.
-    assert w(Q, long, Attn(causal=True, splits=7)) == 3 * 2 * 7 * state(16) + 16
+    # Five rows of two heads a KV head in three sequences: 16 rows a tile, a state and a line of memory for each place of the chip
+    # (the six tiles there may be are fewer).
+    few = w(Q, long, Attn(causal=True))
+    assert few > 0 and few % (state(16) + 128) == 0
+    many = w(t(900, 4, 64), long, Attn(causal=True))  # 128 rows a tile
+    assert many > 0 and (many - 16) % state(128) == 0
+    # A named count: that many states for each tile, three a KV head.
+    assert w(Q, long, Attn(causal=True, splits=7)) == 3 * 2 * 7 * (state(16) + 128)
     assert w(Q, short, Attn(causal=True, splits=7)) == 0  # no more splits than key blocks: one
     # What the op would not take asks for nothing.
     assert w(t(5, 3, 64), long, Attn()) == 0 and w(Q, long, Attn(keys=KeyMask.lens(t(3, dtype=I32)))) == 0
