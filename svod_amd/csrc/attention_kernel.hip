@@ -690,7 +690,7 @@ __device__ __forceinline__ void flash_fwd_body(
     }
     for (; blk < my_end; blk++) edge_step<D, NW, CAUSAL>(w, smem, blk, my_end, sv, bm, seen);
   }
-  for (; blk < (SIDES == 2 ? steps : end); blk++) idle_step<D, NW>(w, smem, blk);
+  for (; blk < (SIDES == 2 ? steps : end); blk++) idle_step<D, NW>(w, blk);
 
   // ---- the appended rows (L739-755, L827-846): one more block of keys, from their own tensors,
   // which only the last split scores; the first `seen` of them are visible and no other mask
@@ -1191,7 +1191,7 @@ __global__ __launch_bounds__(NW * 64, 3) void flash_stream_kernel(
     // Steps with nothing to compute: a causal wave past its diagonal, and the padding of an odd
     // item, which keeps the next item's blocks in the slots a first item's would be in.
     const int steps = more_items ? w.end_even : end;
-    for (; blk < steps; blk++) idle_step<D, NW>(w, smem, blk);
+    for (; blk < steps; blk++) idle_step<D, NW>(w, blk);
 
     // ---- out = o / (l == 0 ? 1 : l), bounded store (L892-898, L974-980).  The stores fly under
     // the next item's first step.

@@ -228,8 +228,6 @@ template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot);
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot);
-template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void land_pages(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk, int par);
 
 // The fills are issued as raw instructions: the compiler's wait-count pass treats an LDS fill
 // it knows about as aliasing every later LDS read and would park the wave on the NEXT tile's
@@ -632,8 +630,8 @@ __device__ __forceinline__ void hot_step(Wave<D, NW, F16, FLAGS> &w, const uint8
     bm = __builtin_fmaxf(p.a, p.b);
   }
   w.l_run = w.l_run * corr + ((bs[0] + bs[1]) + (bs[2] + bs[3]));
-  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, PAR);
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
+  // vmcnt(0): the fills issued this step have landed.  (Codes are in registers, for the next step to write.)
+  if constexpr ((FLAGS & kCoded) == 0) __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 }
 
@@ -689,19 +687,18 @@ __device__ __forceinline__ void edge_step(Wave<D, NW, F16, FLAGS> &w, const uint
       bm = row_max(sv);
     }
   }
-  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, const_cast<uint8_t *>(smem), blk, par);
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the fills issued this step have landed
+  // vmcnt(0): the fills issued this step have landed.  (Codes are in registers, for the next step to write.)
+  if constexpr ((FLAGS & kCoded) == 0) __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 }
 
 // A step of a wave with nothing to compute: fills and the barrier only.
 template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void idle_step(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk) {
+__device__ __forceinline__ void idle_step(Wave<D, NW, F16, FLAGS> &w, int blk) {
   const int par = blk & 1;
   fill_v<D, NW>(w, blk + 1, par ^ 1);
   fill_k<D, NW>(w, blk + 2, par);
-  if constexpr ((FLAGS & kCoded) != 0) land_pages<D, NW>(w, smem, blk, par);
-  __builtin_amdgcn_s_waitcnt(0x0f70);
+  if constexpr ((FLAGS & kCoded) == 0) __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
 }
 

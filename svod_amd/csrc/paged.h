@@ -201,17 +201,32 @@ struct Place {
   Sequence s;
   bool found;
 };
-// The part of number `at`; or, with BY_ROW, the tile of packed row `at`.
-template <bool BY_ROW>
+// Rows up to which a tile is a stream of keys (paged_few.h), whatever the call's form.
+constexpr int kFewRows = 16;
+// The part of number `at`; or, with BY_ROW, the tile of packed row `at`.  CHUNKS: the parts of sequences of more than kFewRows
+// rows come first.  They are what holds such a launch, and at its front they get compute units of their own, and those of
+// few rows the places beside them.
+template <bool BY_ROW, bool CHUNKS>
 __device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p, int at, const Demand &first, const Parts &all) {
   const int lane = lane_id();
   Place x{};
-  int before = 0;
+  const int few = CHUNKS ? (int)over(kFewRows, (uint32_t)p.group, p.group_rcp) : 0;  // tokens
+  auto in_front = [&](const Demand &d) { return CHUNKS && d.fresh > few; };
+  int chunks = 0;  // the parts in front
+  if (CHUNKS)
+    for (int base = 0; base < deal.batch; base += 64) {
+      const Demand d = base == 0 ? first : demand_of(deal, base + lane);
+      chunks += last_lane(sum_to(in_front(d) ? d.tiles * parts_of(p, d.blocks, all) : 0));
+    }
+  int before_front = 0, before = chunks;
   for (int base = 0; base < deal.batch; base += 64) {
     const Demand d = base == 0 ? first : demand_of(deal, base + lane);
-    const int parts = parts_of(p, d.blocks, all), sum = d.tiles * parts, to = sum_to(sum);
+    const int parts = parts_of(p, d.blocks, all), sum = d.tiles * parts;
+    const bool front = in_front(d);
+    const int to = before + sum_to(front ? 0 : sum), to_front = CHUNKS ? before_front + sum_to(front ? sum : 0) : 0;
+    const int end = front ? to_front : to;  // of the lane's own parts
     const uint64_t here = BY_ROW ? __builtin_amdgcn_ballot_w64(d.start <= at && at - d.start < d.fresh)
-                                 : __builtin_amdgcn_ballot_w64(to > at - before);
+                                 : __builtin_amdgcn_ballot_w64(end > at && end - sum <= at);
     if (here != 0) {
       const int at_lane = __builtin_ctzll(here);
       x.b = base + at_lane;
@@ -219,7 +234,7 @@ __device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p
       x.s.start = __builtin_amdgcn_readlane(d.start, at_lane);
       x.s.fresh = __builtin_amdgcn_readlane(d.fresh, at_lane);
       x.s.len = __builtin_amdgcn_readlane(d.len, at_lane);
-      const int tiles = __builtin_amdgcn_readlane(d.tiles, at_lane), start = before + __builtin_amdgcn_readlane(to - sum, at_lane);
+      const int tiles = __builtin_amdgcn_readlane(d.tiles, at_lane), start = __builtin_amdgcn_readlane(end - sum, at_lane);
       int order;  // the last tile, which sees the most keys, comes first
       if (BY_ROW) {
         x.tile = (int)over((uint32_t)(at - x.s.start), (uint32_t)deal.tokens, deal.tokens_rcp);
@@ -234,7 +249,8 @@ __device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p
       x.found = true;
       return x;
     }
-    before += last_lane(to);
+    before = last_lane(to);
+    if (CHUNKS) before_front = last_lane(to_front);
   }
   return x;
 }
@@ -289,11 +305,11 @@ struct Work {
   int first, end;        // its key blocks
   int tile_first, last;  // the tile's first token, and its last, of the sequence's new ones
 };
-template <bool SHARES>
+template <bool SHARES, bool CHUNKS>
 __device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p, const Turn &t) {
   Work w{};
   w.kvh = t.kvh;
-  w.at = place_of<false>(deal, p, t.at, t.first, t.parts);
+  w.at = place_of<false, CHUNKS>(deal, p, t.at, t.first, t.parts);
   if (!w.at.found) return w;
   w.taken = SHARES ? min(w.at.parts - w.at.part, t.to - t.at) : 1;
   w.whole = w.taken == w.at.parts;

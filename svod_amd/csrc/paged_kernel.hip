@@ -28,6 +28,7 @@
 #endif
 #include "attention_step.h"
 #include "paged.h"
+#include "paged_few.h"
 
 namespace svodk {
 namespace {
@@ -59,6 +60,7 @@ struct PagesOf {
     uint32_t scale[kCodes ? kFills : 1];
   };
   Stage k_stage, v_stage;
+  uint8_t *ring;
 
   __device__ int row_of(int r) const { return run_row + r * kStride * kPer; }
   // The runs of block `n` of the frame.
@@ -139,29 +141,30 @@ __device__ __forceinline__ void land_stage(const Wave<D, NW, F16, FLAGS> &w, uin
     *reinterpret_cast<u32x4 *>(at + (dst[i % P::kPer] ^ 16)) = hi;
   }
 }
+// Codes are asked for a step ahead of their place in the ring: a step writes what the one before asked for, and asks for the next block's.
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
   if (n >= w.end) return;
-  w.pages.find(n);
-  if constexpr ((FLAGS & kCoded) != 0)
-    stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n, w.pages.k_src, w.pages.k_stage);
-  else
+  if constexpr ((FLAGS & kCoded) != 0) {
+    land_stage<D, NW>(w, w.pages.ring + slot * Tile<D>::kBytes, w.pages.k_dst, w.pages.k_stage);
+    if (n + 1 >= w.end) return;
+    w.pages.find(n + 1);
+    stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n + 1, w.pages.k_src, w.pages.k_stage);
+  } else {
+    w.pages.find(n);
     fill_pages<D, NW>(w, w.k_base, n, w.lds0 + slot * Tile<D>::kBytes, w.pages.k_src);
+  }
 }
 // A block's values come a step behind its keys, which have named its runs.
 template <int D, int NW, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, int slot) {
   if (n >= w.end) return;
-  if constexpr ((FLAGS & kCoded) != 0)
-    stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n, w.pages.v_src, w.pages.v_stage);
-  else
+  if constexpr ((FLAGS & kCoded) != 0) {
+    land_stage<D, NW>(w, w.pages.ring + (2 + slot) * Tile<D>::kBytes, w.pages.v_dst, w.pages.v_stage);
+    if (n + 1 < w.end) stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n + 1, w.pages.v_src, w.pages.v_stage);
+  } else {
     fill_pages<D, NW>(w, w.v_base, n, w.lds0 + (2 + slot) * Tile<D>::kBytes, w.pages.v_src);
-}
-// The end of step `blk`: what its fills asked for goes into the ring, V(blk + 1) and K(blk + 2).
-template <int D, int NW, bool F16, unsigned FLAGS>
-__device__ __forceinline__ void land_pages(Wave<D, NW, F16, FLAGS> &w, uint8_t *smem, int blk, int par) {
-  if (blk + 1 < w.end) land_stage<D, NW>(w, smem + (2 + (par ^ 1)) * Tile<D>::kBytes, w.pages.v_dst, w.pages.v_stage);
-  if (blk + 2 < w.end) land_stage<D, NW>(w, smem + par * Tile<D>::kBytes, w.pages.k_dst, w.pages.k_stage);
+  }
 }
 
 template <int D, int NW, bool F16, bool CODED>
@@ -235,16 +238,28 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
     w.qf[ks] = x;
   }
   if constexpr (CODED) {
+    w.pages.ring = smem;
     typename P::Stage ahead;
-    fill_k<D, NW>(w, 0, 0);
-    fill_v<D, NW>(w, 0, 0);
+    auto k_of = [&](int n, typename P::Stage &stage) { stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n, w.pages.k_src, stage); };
+    auto v_of = [&](int n) { stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n, w.pages.v_src, w.pages.v_stage); };
+    if (end > 0) {
+      w.pages.find(0);
+      k_of(0, w.pages.k_stage);
+      v_of(0);
+    }
     if (end > 1) {
       w.pages.find(1);
-      stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, 1, w.pages.k_src, ahead);
+      k_of(1, ahead);
     }
     if (end > 0) {
       land_stage<D, NW>(w, smem, w.pages.k_dst, w.pages.k_stage);
       land_stage<D, NW>(w, smem + 2 * TL::kBytes, w.pages.v_dst, w.pages.v_stage);
+    }
+    // V(1) and K(2), which the first step writes.
+    if (end > 1) v_of(1);
+    if (end > 2) {
+      w.pages.find(2);
+      k_of(2, w.pages.k_stage);
     }
     if (end > 1) land_stage<D, NW>(w, smem + TL::kBytes, w.pages.k_dst, ahead);
   } else {
@@ -271,7 +286,7 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
 #pragma unroll
   for (int db = 0; db < DB; db++) w.acc[db] = zero;
 
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  if constexpr (!CODED) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
 
   // ---- the key loop: blocks [0, my_end) are this wave's, [0, full) of them crossed by no edge of its rows.
@@ -305,7 +320,7 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
     hot_step<D, NW, 1>(w, smem, blk + 1, nv, sv, bm);
   }
   for (; blk < my_end; blk++) edge_step<D, NW, false>(w, smem, blk, my_end, sv, bm, seen);
-  for (; blk < end; blk++) idle_step<D, NW>(w, smem, blk);
+  for (; blk < end; blk++) idle_step<D, NW>(w, blk);
 
   const Pair lp = both_halves(w.l_run);
   const float l_tot = lp.a + lp.b;
@@ -353,8 +368,14 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void paged_kernel(SVODK_
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const Deal deal = SVODK_DEAL;
-  const Work work = work_of<false>(deal, p, turn_of<false>(deal, p));
-  if (work.some) paged_item<D, NW, F16, CODED>(smem, deal, p, work);
+  const Work work = work_of<false, true>(deal, p, turn_of<false>(deal, p));
+  if (!work.some) return;
+  // A sequence of few rows beside chunks is a stream of keys here too: one wave of four with rows would take a step a block.  (30
+  // tokens beside two chunks of 1001 in a window of 1024, e4m3: 52.5 us without, 44.4 with this and the chunks in front.)
+  if (work.whole && (work.last - work.tile_first + 1) * p.group <= kFewRows)
+    few::item<D, 1, F16, CODED, false>(smem, deal, p, work);
+  else
+    paged_item<D, NW, F16, CODED>(smem, deal, p, work);
 #endif
 }
 
@@ -380,7 +401,7 @@ __global__ __launch_bounds__(256) void merge_kernel(SVODK_DEAL_PARAMS, PagedPara
   int row = (int)(from / pieces), piece = (int)(from - (uint32_t)row * pieces), known = -1;
   Place at{};
   for (int i = 0; i < run && row < deal.rows; i++) {
-    if (row != known) at = place_of<true>(deal, p, row, first_demand, parts);
+    if (row != known) at = place_of<true, true>(deal, p, row, first_demand, parts);
     known = row;
     const int head = piece * kMergeHeads<D> + lane / kLanes, here = min(head, p.heads - 1);
     const int kvh = (int)over((uint32_t)here, (uint32_t)p.group, p.group_rcp);
