@@ -20,6 +20,8 @@ namespace svodk {
 namespace {
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+typedef __attribute__((ext_vector_type(2))) short s16x2;
 
 constexpr int kWaves = 4;
 
@@ -36,20 +38,29 @@ __device__ __forceinline__ int row_most(int x) {
   return x;
 }
 
-// Eight values of a row of LANES lanes as codes; `e` the row's exponent.
+// The largest magnitude of eight values' bits, those that are not finite left out with FINITE.
+template <bool F16, bool FINITE>
+__device__ __forceinline__ int most_of(const u32x4 &w) {
+  constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+  u16x2 most = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    u16x2 x = __builtin_bit_cast(u16x2, (uint32_t)(w[i] & 0x7fff7fffu));
+    if constexpr (FINITE) x = u16x2{x[0] < kInf ? x[0] : (uint16_t)0, x[1] < kInf ? x[1] : (uint16_t)0};
+    most = __builtin_elementwise_max(most, x);
+  }
+  return max((int)most[0], (int)most[1]);
+}
+// Eight values of a row of LANES lanes as codes; `e` the row's exponent.  The hardware's conversion divides by the power of two and
+// rounds once, to the nearest even; what is not finite becomes e4m3's NaN.  (Over all values of either type and exponents from -100 to
+// 100 it gives the codes of x * 2^-e.)
 template <bool F16, int LANES>
 __device__ __forceinline__ u32x2 to_codes(const u32x4 &w, int &e) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr uint32_t kInf = F16 ? 0x7c00u : 0x7f80u;
+  constexpr int kInf = F16 ? 0x7c00 : 0x7f80;
   constexpr int kTop = F16 ? 8 : 120;  // with it a code of 256 is past the type's largest value
-  int most = 0;  // the largest finite magnitude's bits
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
-    most = max(most, (int)(lo < kInf ? lo : 0u));
-    most = max(most, (int)(hi < kInf ? hi : 0u));
-  }
-  most = row_most<LANES>(most);
+  int most = row_most<LANES>(most_of<F16, false>(w));
+  if (__builtin_amdgcn_ballot_w64(most >= kInf) != 0) most = row_most<LANES>(most_of<F16, true>(w));
   uint32_t bits;  // as an f32's
   if constexpr (F16)
     bits = __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)most));
@@ -57,45 +68,65 @@ __device__ __forceinline__ u32x2 to_codes(const u32x4 &w, int &e) {
     bits = (uint32_t)most << 16;
   // 448 = 1.75 * 2^8: one more where the significand is past 1.75.
   e = max((int)((bits + 0x1fffffu) >> 23) - 135, -117);
-  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-  const float limit = e >= kTop ? 240.0f : 448.0f;
-  float x[8];
-  widen<F16>(w, x);
-  uint32_t out[2];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    // A value that is not finite is left out of the clamp and made NaN: e4m3 has no infinity.
-    const uint32_t half = (i & 1) ? (w[i / 2] >> 16) & 0x7fffu : w[i / 2] & 0x7fffu;
-    const float y = __builtin_fminf(__builtin_fmaxf(x[i] * down, -limit), limit);
-    x[i] = half < kInf ? y : __uint_as_float(0x7fc00000u);
-  }
+  const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
+  u32x2 out;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    int word = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-    word = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], word, true);
-    out[i] = (uint32_t)word;
+    s16x2 c = {0, 0};
+    const uint32_t lo = w[2 * i], hi = w[2 * i + 1];
+    if constexpr (F16) {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(f16x2, lo), scale, false);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(f16x2, hi), scale, true);
+    } else {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, lo), scale, false);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, hi), scale, true);
+    }
+    out[i] = __builtin_bit_cast(uint32_t, c);
   }
-  return u32x2{out[0], out[1]};
+  if (__builtin_amdgcn_ballot_w64(e >= kTop) != 0) {
+    // 240 (0x77) in the place of 256 and more, NaN (0x7f) apart.
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t code = (out[i] >> (8 * j)) & 0xffu, size = code & 0x7fu;
+        word |= (e >= kTop && size > 0x77u && size < 0x7fu ? (code & 0x80u) | 0x77u : code) << (8 * j);
+      }
+      out[i] = word;
+    }
+  }
+  return out;
 #else
   return u32x2{};
 #endif
 }
 
-// ---- into the pages.  A wave takes 64 / LANES packed rows of one KV head, keys and values.
-template <int D, bool F16, bool CODED>
-__global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v) {
+// ---- into the pages.  A wave takes 64 / LANES packed rows, keys and values, of HEADS KV heads one after the other: four where
+// there are waves enough, so that a wave has eight loads on their way while it looks its rows up, and looks them up once (13312
+// rows of 8 heads of 128 into codes 25.2 us a head a wave with the codes by arithmetic, 18.2 so; eight
+// prompts of up to 2047 tokens in f16, 20 heads of 64, 26.4 and 25.5).
+template <int D, bool F16, bool CODED, int HEADS>
+__global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, uint32_t strips, const uint16_t *__restrict__ k,
+                                                                  const uint16_t *__restrict__ v) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;
   const int lane = (int)__builtin_amdgcn_workitem_id_x() & 63;
   const uint32_t wave = __builtin_amdgcn_workgroup_id_x() * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)__builtin_amdgcn_workitem_id_x() >> 6);
-  const uint32_t group = wave / (uint32_t)p.kv_heads;
-  const int head = (int)(wave - group * (uint32_t)p.kv_heads);
+  const uint32_t group = wave / strips;
+  const int head0 = (int)(wave - group * strips) * HEADS;
   const int64_t row0 = (int64_t)group * kRows;
   if (row0 >= p.rows) return;
   const int64_t row = row0 + lane / kLanes;
   const bool there = row < p.rows;
-  const int64_t from = ((there ? row : row0) * p.kv_heads + head) * D + lane % kLanes * 8;
-  const u32x4 xk = *reinterpret_cast<const u32x4 *>(k + from), xv = *reinterpret_cast<const u32x4 *>(v + from);
+  const int column = lane % kLanes * 8;
+  u32x4 xk[HEADS], xv[HEADS];
+#pragma unroll
+  for (int h = 0; h < HEADS; h++) {
+    // A row or head past the last loads one that is there, and drops it.
+    const int64_t from = ((there ? row : row0) * p.kv_heads + min(head0 + h, p.kv_heads - 1)) * D + column;
+    xk[h] = *reinterpret_cast<const u32x4 *>(k + from), xv[h] = *reinterpret_cast<const u32x4 *>(v + from);
+  }
   // The sequence and the position of each of the wave's rows: the sequences a lane each, 64 at a time.
   int b = -1, at = -1;
   for (int base = 0; base < p.batch; base += 64) {
@@ -115,20 +146,27 @@ __global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, c
     }
     if (found == kRows) break;
   }
-  if (!there || b < 0 || at < 0) return;  // a row of no sequence, or past what the length has room for
-  const int64_t to = page_row(p, page_at(p, b, at >> p.page_log2), head) + (at & ((1 << p.page_log2) - 1));
-  if constexpr (CODED) {
-    int ek, ev;
-    const u32x2 ck = to_codes<F16, kLanes>(xk, ek), cv = to_codes<F16, kLanes>(xv, ev);
-    *reinterpret_cast<u32x2 *>((uint8_t *)p.k + to * D + lane % kLanes * 8) = ck;
-    *reinterpret_cast<u32x2 *>((uint8_t *)p.v + to * D + lane % kLanes * 8) = cv;
-    if (lane % kLanes == 0) {
-      ((uint8_t *)p.k_scale)[to] = (uint8_t)(ek + 127);
-      ((uint8_t *)p.v_scale)[to] = (uint8_t)(ev + 127);
+  // A row of no sequence, or past what the length has room for, goes nowhere; its lanes go on, for their neighbours' sums.
+  const bool goes = there && b >= 0 && at >= 0;
+  const int page = goes ? page_at(p, b, at >> p.page_log2) : 0, in_page = at & ((1 << p.page_log2) - 1);
+#pragma unroll
+  for (int h = 0; h < HEADS; h++) {
+    const bool writes = goes && head0 + h < p.kv_heads;
+    const int64_t to = page_row(p, page, head0 + h) + in_page;
+    if constexpr (CODED) {
+      int ek, ev;
+      const u32x2 ck = to_codes<F16, kLanes>(xk[h], ek), cv = to_codes<F16, kLanes>(xv[h], ev);
+      if (!writes) continue;
+      *reinterpret_cast<u32x2 *>((uint8_t *)p.k + to * D + column) = ck;
+      *reinterpret_cast<u32x2 *>((uint8_t *)p.v + to * D + column) = cv;
+      if (column == 0) {
+        ((uint8_t *)p.k_scale)[to] = (uint8_t)(ek + 127);
+        ((uint8_t *)p.v_scale)[to] = (uint8_t)(ev + 127);
+      }
+    } else if (writes) {
+      *reinterpret_cast<u32x4 *>((uint16_t *)p.k + to * D + column) = xk[h];
+      *reinterpret_cast<u32x4 *>((uint16_t *)p.v + to * D + column) = xv[h];
     }
-  } else {
-    *reinterpret_cast<u32x4 *>((uint16_t *)p.k + to * D + lane % kLanes * 8) = xk;
-    *reinterpret_cast<u32x4 *>((uint16_t *)p.v + to * D + lane % kLanes * 8) = xv;
   }
 #endif
 }
@@ -171,11 +209,19 @@ __global__ __launch_bounds__(kWaves * 64) void read_pages_kernel(PagesArgs p, in
 #endif
 }
 
+template <int D, bool F16, bool CODED, int HEADS>
+hipError_t write_heads(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) {
+  const int64_t groups = ((int64_t)a.rows * D / 8 + 63) / 64, strips = (a.kv_heads + HEADS - 1) / HEADS;
+  const int64_t grid = (groups * strips + kWaves - 1) / kWaves;
+  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
+  return Launch<write_pages_kernel<D, F16, CODED, HEADS>>::run(grid, kWaves * 64, 0, 0, stream, a, (uint32_t)strips, (const uint16_t *)k,
+                                                               (const uint16_t *)v);
+}
 template <int D, bool F16, bool CODED>
 hipError_t write(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) {
-  const int64_t groups = ((int64_t)a.rows * D / 8 + 63) / 64, waves = groups * a.kv_heads, grid = (waves + kWaves - 1) / kWaves;
-  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
-  return Launch<write_pages_kernel<D, F16, CODED>>::run(grid, kWaves * 64, 0, 0, stream, a, (const uint16_t *)k, (const uint16_t *)v);
+  // Four heads a wave from eight waves a compute unit on that have four.
+  const bool many = ((int64_t)a.rows * D / 8 + 63) / 64 * (a.kv_heads / 4) >= 256 * 8;
+  return many ? write_heads<D, F16, CODED, 4>(a, k, v, stream) : write_heads<D, F16, CODED, 1>(a, k, v, stream);
 }
 template <int D, bool F16, bool CODED>
 hipError_t read(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream) {
