@@ -250,7 +250,7 @@ int svodk_order_rows(const svodk_tensor *keys, const svodk_tensor *order, void *
  */
 typedef struct svodk_pages {
   const svodk_tensor *k, *v;             /* [pages, kv_heads, page, D], one type */
-  const svodk_tensor *k_scale, *v_scale; /* [pages, kv_heads, page] SVODK_E8M0 with pools of SVODK_E4M3, else NULL */
+  const svodk_tensor *k_scale, *v_scale; /* [pages, kv_heads, page] SVODK_E8M0 with pools of SVODK_E4M3, else NULL; bytes 1 to 254 */
   const svodk_tensor *table;             /* [B, columns] I32; entries past a sequence's pages are not used */
   const svodk_tensor *lens;              /* [B] I32 or I64 */
   const svodk_tensor *starts;            /* [B + 1] I32 or I64, ascending */

@@ -282,6 +282,11 @@ struct Sharers {
   int first, last;    // workgroups of the KV head
   int64_t slot, next; // the first one's, and the second one's
   int step;           // from there on
+  // Whether all of them are in the launch, with slots.  (Starts that descend give more tiles than there are rows, whose last have none.  A tile
+  // that some could count themselves in for and others not would leave its word between two counts for the next replay.)
+  __device__ bool fit(int slots) const {
+    return first >= 0 && last >= first && (last == first ? slot : next + (int64_t)(last - first - 1) * step) < slots;
+  }
 };
 __device__ __forceinline__ Sharers sharers_of(const Deal &deal, const Place &at, int kvh, const Parts &parts) {
   Sharers x;
@@ -318,7 +323,7 @@ __device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p, 
     w.sharers = sharers_of(deal, w.at, t.kvh, t.parts);
     const int which = t.mine - w.sharers.first;
     w.slot = which == 0 ? w.sharers.slot : w.sharers.next + (int64_t)(which - 1) * w.sharers.step;
-    w.some = w.slot < p.slots;  // (there is no room: starts that descend give more rows than there are)
+    w.some = w.sharers.fit(p.slots);
   }
   const Sequence &s = w.at.s;
   w.tile_first = w.at.tile * deal.tokens;
@@ -347,6 +352,11 @@ __device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p, 
   w.first = uniform(first);
   w.end = uniform(end);
   return w;
+}
+
+// The first key that a row of the tile sees.
+__device__ __forceinline__ int lowest_key(const PagedParams &p, const Work &w) {
+  return p.win_left >= 0 ? max(0, w.at.s.base() + w.tile_first - p.win_left) : 0;
 }
 
 // A lane's query row of a tile: query head row % group of the KV head's, of the tile's token row / group.  The keys [lo, hi] it

@@ -171,18 +171,20 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
   const int hi_least = __builtin_amdgcn_readlane(hi[0], 0), lo_most = __builtin_amdgcn_readlane(lo[RT - 1], 15);
 
   // ---- the loads of a block: its keys' rows by runs of 16, none of which lies in two pages.  Keys past the length read as
-  // zeros (a page's last rows hold anything, and 0 times that is not 0), and so does all of a block past the item's last: no load stands
-  // under a branch, where the wait for one would be a wait for all.
+  // zeros (a page's last rows hold anything, and 0 times that is not 0), and so does a run in front of the window (whose page the
+  // sequence may have given away) and all of a block past the item's last: no load stands under a branch, where the wait for one would be
+  // a wait for all.
   int64_t run[4];
   int left[4];
-  auto find = [&](int n) {
+  auto find = [&](int n, bool first) {  // first: the wave's, which alone may hold keys in front of the window
     const int key0 = first_key + n * kKeys;
     ids.go(key0 >> p.page_log2);
+    const int lowest = first ? __builtin_amdgcn_readfirstlane(lo[0]) : 0;  // that a row of the tile sees
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const int key = key0 + 16 * r;
       run[r] = (int64_t)((uint64_t)(uint32_t)ids.of(key >> p.page_log2) * page_rows) + (key & ((1 << p.page_log2) - 1));
-      left[r] = n < end ? min(max(len - n * kKeys - 16 * r, 0), 16) : 0;
+      left[r] = n < end && (!first || n * kKeys + 16 * r + 16 > lowest) ? min(max(len - n * kKeys - 16 * r, 0), 16) : 0;
     }
   };
   u32x4 kf[4][KL], vf[4][kVPer];
@@ -223,7 +225,7 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
   const bool counts = !whole && wave == 0 && lane == 0;
   uint64_t found = 0;
   if (counts) found = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  find(wave);
+  find(wave, true);
   ask_k();
   ask_v();
 
@@ -277,7 +279,7 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
       }
     }
     // The next block's keys are on their way from here on.
-    find(n + kWaves);
+    find(n + kWaves, false);
     ask_k();
 
     // ---- the softmax's step, a row in four lanes.

@@ -51,6 +51,7 @@ struct PagesOf {
   int page_log2;
   uint32_t page_rows;                // rows of a page, all KV heads'
   int first_key;                     // the frame's
+  int lowest;                        // the first key that a row of the tile sees
   int64_t run[kRuns];                // the pool's row that each of this wave's runs of the block filled last starts at
   int run_row;                       // the first run's row of the block
   int k_src[kPer], v_src[kPer];      // a lane's offset in a run's descriptor (straight into LDS: swizzled)
@@ -63,6 +64,13 @@ struct PagesOf {
   uint8_t *ring;
 
   __device__ int row_of(int r) const { return run_row + r * kStride * kPer; }
+  // The rows that run r of block n has for the tile, whose keys end at `len`.  None of 16 in front of a window, which are the first
+  // block's: a sequence may have given pages away that its window has left.
+  template <bool FIRST>
+  __device__ int rows_of(int n, int r, int len) const {
+    const int key = n * kBkv + row_of(r);
+    return !FIRST || key + 16 > lowest ? min(max(len - key, 0), 16) : 0;
+  }
   // The runs of block `n` of the frame.
   __device__ void find(int n) {
     const int key0 = first_key + n * kBkv;
@@ -88,13 +96,13 @@ struct Pages<D, NW, kPaged | kCoded> : PagesOf<D, NW, kPaged | kCoded> {};
 
 // This wave's share of block `n` from the pool at `base`, whose runs find() has named, straight into LDS: keys past the length
 // land as zeros (a page's last rows hold anything, and 0 times that is not 0).
-template <int D, int NW, bool F16, unsigned FLAGS>
+template <int D, int NW, bool FIRST, bool F16, unsigned FLAGS>
 __device__ __forceinline__ void fill_pages(const Wave<D, NW, F16, FLAGS> &w, const uint8_t *base, int n, int lds_at,
                                            const int *src) {
   using P = decltype(w.pages);
 #pragma unroll
   for (int r = 0; r < P::kRuns; r++) {
-    const int left = min(max(w.len - n * kBkv - w.pages.row_of(r), 0), 16);
+    const int left = w.pages.template rows_of<FIRST>(n, r, w.len);
     const i32x4 rsrc = rows_rsrc(base + w.pages.run[r] * P::kRowBytes, left, P::kRowBytes);
 #pragma unroll
     for (int j = 0; j < P::kPer; j++)
@@ -105,14 +113,14 @@ __device__ __forceinline__ void fill_pages(const Wave<D, NW, F16, FLAGS> &w, con
   }
 }
 // The same of codes: into registers, with their rows' scales.
-template <int D, int NW, bool F16, unsigned FLAGS, typename S>
+template <int D, int NW, bool FIRST, bool F16, unsigned FLAGS, typename S>
 __device__ __forceinline__ void stage_pages(const Wave<D, NW, F16, FLAGS> &w, const uint8_t *base, const uint8_t *scales, int n,
                                             const int *src, S &stage) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using P = decltype(w.pages);
 #pragma unroll
   for (int r = 0; r < P::kRuns; r++) {
-    const int left = min(max(w.len - n * kBkv - w.pages.row_of(r), 0), 16);
+    const int left = w.pages.template rows_of<FIRST>(n, r, w.len);
     const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + w.pages.run[r] * P::kRowBytes), 0,
                                                         left * P::kRowBytes, 0x00020000);
 #pragma unroll
@@ -149,10 +157,10 @@ __device__ __forceinline__ void fill_k_pages(Wave<D, NW, F16, FLAGS> &w, int n, 
     land_stage<D, NW>(w, w.pages.ring + slot * Tile<D>::kBytes, w.pages.k_dst, w.pages.k_stage);
     if (n + 1 >= w.end) return;
     w.pages.find(n + 1);
-    stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n + 1, w.pages.k_src, w.pages.k_stage);
+    stage_pages<D, NW, false>(w, w.k_base, w.pages.k_scale, n + 1, w.pages.k_src, w.pages.k_stage);
   } else {
     w.pages.find(n);
-    fill_pages<D, NW>(w, w.k_base, n, w.lds0 + slot * Tile<D>::kBytes, w.pages.k_src);
+    fill_pages<D, NW, false>(w, w.k_base, n, w.lds0 + slot * Tile<D>::kBytes, w.pages.k_src);
   }
 }
 // A block's values come a step behind its keys, which have named its runs.
@@ -161,9 +169,9 @@ __device__ __forceinline__ void fill_v_pages(Wave<D, NW, F16, FLAGS> &w, int n, 
   if (n >= w.end) return;
   if constexpr ((FLAGS & kCoded) != 0) {
     land_stage<D, NW>(w, w.pages.ring + (2 + slot) * Tile<D>::kBytes, w.pages.v_dst, w.pages.v_stage);
-    if (n + 1 < w.end) stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n + 1, w.pages.v_src, w.pages.v_stage);
+    if (n + 1 < w.end) stage_pages<D, NW, false>(w, w.v_base, w.pages.v_scale, n + 1, w.pages.v_src, w.pages.v_stage);
   } else {
-    fill_pages<D, NW>(w, w.v_base, n, w.lds0 + (2 + slot) * Tile<D>::kBytes, w.pages.v_src);
+    fill_pages<D, NW, false>(w, w.v_base, n, w.lds0 + (2 + slot) * Tile<D>::kBytes, w.pages.v_src);
   }
 }
 
@@ -213,6 +221,7 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
   w.pages.page_log2 = p.page_log2;
   w.pages.page_rows = (uint32_t)deal.kv_heads << p.page_log2;
   w.pages.first_key = first_key;
+  w.pages.lowest = lowest_key(p, work) - first_key;
   w.pages.run_row = (w.wave * P::kRows) & ~15;
   w.pages.ids.begin(p, work.at.b, first_key >> p.page_log2);
 #pragma unroll
@@ -240,12 +249,12 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
   if constexpr (CODED) {
     w.pages.ring = smem;
     typename P::Stage ahead;
-    auto k_of = [&](int n, typename P::Stage &stage) { stage_pages<D, NW>(w, w.k_base, w.pages.k_scale, n, w.pages.k_src, stage); };
-    auto v_of = [&](int n) { stage_pages<D, NW>(w, w.v_base, w.pages.v_scale, n, w.pages.v_src, w.pages.v_stage); };
+    auto k_of = [&](int n, typename P::Stage &stage) { stage_pages<D, NW, false>(w, w.k_base, w.pages.k_scale, n, w.pages.k_src, stage); };
+    auto v_of = [&](int n) { stage_pages<D, NW, false>(w, w.v_base, w.pages.v_scale, n, w.pages.v_src, w.pages.v_stage); };
     if (end > 0) {
       w.pages.find(0);
-      k_of(0, w.pages.k_stage);
-      v_of(0);
+      stage_pages<D, NW, true>(w, w.k_base, w.pages.k_scale, 0, w.pages.k_src, w.pages.k_stage);
+      stage_pages<D, NW, true>(w, w.v_base, w.pages.v_scale, 0, w.pages.v_src, w.pages.v_stage);
     }
     if (end > 1) {
       w.pages.find(1);
@@ -263,8 +272,11 @@ __device__ __forceinline__ void paged_item(uint8_t *smem, const Deal &deal, cons
     }
     if (end > 1) land_stage<D, NW>(w, smem + TL::kBytes, w.pages.k_dst, ahead);
   } else {
-    fill_k<D, NW>(w, 0, 0);
-    fill_v<D, NW>(w, 0, 0);
+    if (end > 0) {
+      w.pages.find(0);
+      fill_pages<D, NW, true>(w, w.k_base, 0, w.lds0, w.pages.k_src);
+      fill_pages<D, NW, true>(w, w.v_base, 0, w.lds0 + 2 * TL::kBytes, w.pages.v_src);
+    }
     fill_k<D, NW>(w, 1, 1);
   }
 
@@ -407,8 +419,8 @@ __global__ __launch_bounds__(256) void merge_kernel(SVODK_DEAL_PARAMS, PagedPara
     const int kvh = (int)over((uint32_t)here, (uint32_t)p.group, p.group_rcp);
     const Sharers sharers = sharers_of(deal, at, kvh, parts);
     const int last = at.found ? sharers.last - sharers.first : 0;
-    // (Slots past the workspace's: as work_of().  The branch is the same in all waves.)
-    if (last > 0 && sharers.next + (int64_t)(last - 1) * sharers.step - kvh + deal.kv_heads <= p.slots) {
+    // (No slots: as work_of(), here for all of the lanes' heads.  The branch is the same in all waves.)
+    if (last > 0 && sharers.first >= 0 && sharers.next + (int64_t)(last - 1) * sharers.step - kvh + deal.kv_heads <= p.slots) {
       const int in_tile = (row - at.s.start - at.tile * deal.tokens) * p.group + here - kvh * p.group;
       const int column = lane % kLanes * 8;
       float m = -1e30f, l = 0.0f, acc[8] = {};
@@ -538,6 +550,8 @@ int64_t paged_slots(const PagedArgs &a) {
   if (a.splits > 1) return tiles * a.splits;
   const bool few = paged_tile_rows(a) != 128;
   // Too short to be worth a merge, whatever the lengths; and blocks of all tiles are counted in 31 bits.
+  // (A state for each of many tiles of 128 rows would be gigabytes, where none is more than a small part of the launch.)
+  if (!few && tiles > 4 * places(a)) return 0;
   if (blocks <= (few ? 8 : 4) || tiles / a.pages.kv_heads * blocks > 0x3fffffff || (dense(a) && blocks < (few ? 16 : 64))) return 0;
   return few && dense(a) ? 2 * (places(a) + a.pages.kv_heads) : paged_workgroups(a);
 }

@@ -351,3 +351,291 @@ def test_two_streams_at_once(device):
     for i in range(2):
         for x in got[i]:
             assert torch.equal(bits(x), bits(want[i]))
+
+
+# ---- calls of every form, at their borders.
+def ragged(count, seed, least, most):
+    r = np.random.default_rng(seed)
+    return [int(x) for x in r.integers(least, most + 1, count)]
+
+
+def both(device, case, h, opts, seed=3, by=1.0):
+    """The call's result held to the reference, and the same bits from a second call."""
+    q = normal((case.rows, h, case.k.shape[3]), case.dtype, seed, device, by)
+    got = svod_amd.attention_paged(q, case.pages, Attn(**opts))
+    held(got, *ref.attention(case, q, **{k: v for k, v in opts.items() if k != "splits"}))
+    assert torch.equal(bits(got), bits(svod_amd.attention_paged(q, case.pages, Attn(**opts))))
+    return svod_amd.chosen()
+
+
+KINDS = [(BF16, False), (F16, False), (BF16, True), (F16, True)]
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+@pytest.mark.parametrize("window", [None, (70, 0), (200, 3)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_chunks_beside_single_tokens(device, d, window, dtype, coded):
+    """More sequences than lanes, a few with chunks between those of one to five tokens: two tile forms in one launch."""
+    context, fresh = ragged(71, d, 0, 300), ragged(71, d + 1, 0, 5)
+    for b, n in ((3, 150), (40, 129), (66, 128), (70, 31)):
+        fresh[b] = n
+    case = make(device, context, fresh, kv_heads=1, d=d, page=32, dtype=dtype, coded=coded, seed=d)
+    assert "rows: 128" in both(device, case, 8, dict(causal=True, window=window))
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+def test_a_long_sequence_among_many_is_split(device, dtype, coded):
+    """Tiles for more than half of the places and one sequence far longer than the others: of 128 rows its own alone is split."""
+    fresh = [128] * 70 + [1, 130]
+    context = ragged(70, 5, 0, 64) + [20000, 9000]
+    case = make(device, context, fresh, kv_heads=2, d=64, page=64, dtype=dtype, coded=coded, seed=9)
+    q = normal((case.rows, 4, 64), dtype, 3, device)
+    assert svod_amd.attention_paged_workspace(q, case.pages, Attn(causal=True)) > 0
+    assert "rows: 128" in both(device, case, 4, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+@pytest.mark.parametrize("d,h,hkv,fresh", [(64, 4, 4, 1), (128, 8, 4, 1), (64, 8, 4, 5), (128, 16, 4, 6)])
+def test_shares_of_many_ragged_sequences(device, d, h, hkv, fresh, dtype, coded):
+    """Few rows a sequence, more tiles than half of the places, lengths that differ much: every place takes an even share of all
+    blocks, which begins and ends inside tiles, and tiles lie in the shares of one to many places."""
+    context = ragged(150, d, 0, 150)
+    context[7], context[80], context[149] = 9000, 4000, 6000
+    case = make(device, context, [1 + b % fresh for b in range(150)], kv_heads=hkv, d=d, page=16, dtype=dtype, coded=coded, seed=d + h)
+    assert "rows: 128" not in both(device, case, h, dict(causal=True))
+
+
+@pytest.mark.parametrize("group,tokens,d", [(1, 16, 64), (1, 17, 64), (16, 1, 128), (17, 1, 128), (32, 1, 64), (33, 1, 64), (4, 8, 128),
+                                            (4, 9, 128), (5, 3, 128), (16, 1, 256), (17, 1, 256), (127, 1, 128)])
+def test_rows_at_the_forms_borders(device, group, tokens, d):
+    case = make(device, [333, 0, 64, 1000], [tokens] * 4, kv_heads=1, d=d, page=16, seed=group)
+    both(device, case, group, dict(causal=True))
+    both(device, case, group, dict(causal=True, splits=4))
+
+
+@pytest.mark.parametrize("coded", [False, True])
+def test_one_very_long_sequence(device, coded):
+    case = make(device, [150_000], [2], kv_heads=1, d=64, page=256, coded=coded, seed=2)
+    both(device, case, 3, dict(causal=True))
+    case.pages.lens[0] = case.lens[0] = 149_999
+    both(device, case, 3, dict(causal=True, window=(70_000, 0)))
+
+
+def test_more_splits_than_a_merge_takes_at_once(device):
+    """A state a block: a tile of several hundred, of few rows and of 128."""
+    for fresh in (1, 130):
+        case = make(device, [20_000, 70], [fresh, 1], kv_heads=1, d=64, page=64, seed=fresh)
+        both(device, case, 4, dict(causal=True, splits=400))
+
+
+@pytest.mark.parametrize("coded", [False, True])
+@pytest.mark.parametrize("fresh", [[1, 2, 1], [70, 90, 40]])
+def test_pages_in_front_of_the_window_are_not_read(device, coded, fresh):
+    """What a sequence's window has left it may give away: the table's entries there point at a page of NaN, or at none."""
+    window, page = (100, 0), 32
+    case = make(device, [500, 37, 1000], fresh, kv_heads=2, d=64, page=page, coded=coded, seed=4)
+    q = normal((case.rows, 32, 64), BF16, 5, device)
+    opts = Attn(causal=True, window=window)
+    want = svod_amd.attention_paged(q, case.pages, opts)
+    held(want, *ref.attention(case, q, causal=True, window=window))
+    spare = next(i for i in range(case.k.shape[0]) if not bool((case.table == i).any()))
+    for x in (case.pages.k, case.pages.v):
+        x[spare].view(torch.uint8 if coded else torch.int16).fill_(0x7f if coded else 0x7fff)
+    for b, n in enumerate(case.lens):
+        gone = max(0, n - fresh[b] - window[0]) // page
+        case.pages.table[b, :gone] = spare
+        case.pages.table[b, :gone:3] = -1
+    case.pages.table[1, -1] = 0x7fffffff
+    assert torch.equal(bits(want), bits(svod_amd.attention_paged(q, case.pages, opts)))
+
+
+@pytest.mark.parametrize("coded", [False, True])
+def test_pools_past_4_gib(device, coded):
+    """Offsets that pass 32 bits: the pages at both ends of pools of 4.6 GiB."""
+    page, d, hkv = 64, 128, 8
+    count = (9 << 29) // (page * d * hkv * (1 if coded else 2)) + 3
+    case = make(device, [200, 70, 0], [3, 1, 40], kv_heads=hkv, d=d, page=page, coded=coded, seed=6, fill=0.0)
+    small = case.pages
+    ids = torch.arange(case.k.shape[0])
+    at = torch.where(ids % 2 == 0, ids, count - 1 - ids)  # where the small pool's pages stand in the large one
+    pools = [torch.empty((count, *x.shape[1:]), dtype=torch.uint8 if coded else BF16, device=device) for x in (small.k, small.v)]
+    for pool, x in zip(pools, (small.k, small.v)):
+        for i, to in enumerate(at.tolist()):
+            pool[to].copy_(x[i].view(pool.dtype))
+    assert pools[0].numel() * pools[0].element_size() > 1 << 32
+    scales = None
+    if coded:
+        scales = tuple(torch.empty((count, hkv, page), dtype=torch.uint8, device=device) for _ in range(2))
+        for s, x in zip(scales, small.scales):
+            for i, to in enumerate(at.tolist()):
+                s[to].copy_(x[i].view(torch.uint8))
+        pools, scales = [p.view(E4M3) for p in pools], tuple(s.view(E8M0) for s in scales)
+    table = small.table.clone().cpu()
+    used = (table >= 0) & (table < len(ids))
+    table[used] = at[table[used].long()].to(torch.int32)
+    large = Pages(pools[0], pools[1], table.to(device), small.lens, small.starts, scales)
+    q, k = normal((case.rows, 16, d), BF16, 8, device), normal((case.rows, hkv, d), BF16, 9, device, by=3.0)
+    for step in range(2):
+        got, want = (svod_amd.attention_paged(q, p, Attn(causal=True)) for p in (large, small))
+        assert torch.equal(bits(got), bits(want))
+        for a, b in zip(svod_amd.read_pages(large, 210), svod_amd.read_pages(small, 210)):
+            assert torch.equal(bits(a), bits(b))
+        for p in (large, small):
+            svod_amd.write_pages(k, -k, p)
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+def test_many_rows_are_written_as_few_are(device, dtype, coded):
+    """Large calls take four heads a wave, here with one over: the same pages as sequence by sequence, and unlike values too."""
+    hkv, d, page = 13, 128, 64
+    fresh = [1500, 1, 700, 0, 803]
+    big = make(device, [0, 5, 100, 9, 64], fresh, kv_heads=hkv, d=d, page=page, dtype=dtype, coded=coded, seed=7, fill=0.0, rows_before=3, rows_after=2)
+    k, v = (normal((big.rows, hkv, d), dtype, s, device, by=3.0) for s in (1, 2))
+    k[::7] *= 2.0 ** -12
+    k[11, :, 5], k[12, 3, 9], v[13, 12, 127] = float("inf"), float("nan"), -float("inf")
+    v[::5] *= 1000.0
+    one = Pages(big.pages.k.clone(), big.pages.v.clone(), big.pages.table, big.pages.lens, big.pages.starts,
+                tuple(x.clone() for x in big.pages.scales) if coded else None)
+    svod_amd.write_pages(k, v, big.pages)
+    for b in range(5):
+        s, e = big.starts[b], big.starts[b + 1]
+        for at in range(s, e, 400):  # the sequence's rows a few hundred at a time
+            to = min(e, at + 400)
+            lens = torch.tensor([big.lens[b] - (e - to)], dtype=torch.int32, device=device)
+            starts = torch.tensor([0, to - at], dtype=torch.int32, device=device)
+            svod_amd.write_pages(k[at:to].contiguous(), v[at:to].contiguous(),
+                                 Pages(one.k, one.v, one.table[b:b + 1].contiguous(), lens, starts, one.scales))
+    pairs = [(big.pages.k, one.k), (big.pages.v, one.v), *(zip(big.pages.scales, one.scales) if coded else ())]
+    for a, b in pairs:
+        assert torch.equal(bits(a), bits(b))
+
+
+def test_a_shared_prefix(device):
+    """Two sequences over the same first pages, and one that is there twice."""
+    case = make(device, [640, 700, 64], [1, 1, 1], kv_heads=2, d=64, page=64, seed=3)
+    case.table[1, :10] = case.table[0, :10]
+    case.pages.table.copy_(case.table)
+    both(device, case, 4, dict(causal=True))
+    twice = Pages(**{**case.pages.__dict__, "table": case.pages.table[[0, 0, 0]].contiguous(),
+                     "lens": case.pages.lens[[0, 0, 0]].contiguous()})
+    q = normal((1, 4, 64), BF16, 4, device).expand(3, 4, 64).contiguous()
+    got = svod_amd.attention_paged(q, twice, Attn(causal=True))
+    assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2]))
+    k, _ = svod_amd.read_pages(twice, 641)
+    assert torch.equal(bits(k[0]), bits(k[1])) and torch.equal(bits(k[0]), bits(k[2]))
+
+
+def test_two_graphs_and_eager_calls_on_one_workspace(device):
+    """Two captured steps of unlike forms and a call of its own use one workspace in turn; lengths change between the replays, and
+    once the starts are not ascending: what that leaves in the workspace costs the next replay nothing."""
+    opts = Attn(causal=True)
+    cases = [make(device, [2000, 900, 50], [1, 1, 2], kv_heads=2, d=128, page=16, seed=60),
+             make(device, [100] * 97 + [3000, 2500, 40], [1] * 100, kv_heads=8, d=128, page=16, seed=61),
+             make(device, [3000, 20], [140, 1], kv_heads=1, d=128, page=16, seed=62)]
+    heads = (4, 16, 8)
+    qs = [normal((c.rows, h, 128), BF16, 63 + i, device) for i, (c, h) in enumerate(zip(cases, heads))]
+    ws = torch.empty(max(svod_amd.attention_paged_workspace(q, c.pages, opts) for q, c in zip(qs, cases)), dtype=torch.uint8, device=device)
+    assert all(svod_amd.attention_paged_workspace(q, c.pages, opts) > 0 for q, c in zip(qs, cases))
+    outs = [torch.empty_like(q) for q in qs]
+    run = lambda i: svod_amd.attention_paged(qs[i], cases[i].pages, opts, outs[i], ws)
+    stream, graphs = torch.cuda.Stream(), []
+    with torch.cuda.stream(stream):
+        for i in range(3):
+            run(i)
+    torch.cuda.synchronize()
+    for i in range(3):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            run(i)
+    first = [(c.pages.lens.clone(), c.pages.starts.clone()) for c in cases]
+    for turn in range(6):
+        for c, (lens, starts) in zip(cases, first):
+            c.pages.lens.copy_(lens if turn % 2 == 0 else (lens * (turn + 1)) // (turn + 3))
+            c.pages.starts.copy_(starts)
+            if turn == 3:  # wrong: some tiles more than there are rows
+                c.pages.starts[1::2] = 0
+                c.pages.starts[::2] = c.rows
+        for i in (0, 1, 2, 1, 0):
+            outs[i].fill_(9.0)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            if turn == 3:
+                continue
+            got = outs[i].clone()
+            run((i + 1) % 3)  # and the workspace holds something else
+            want = svod_amd.attention_paged(qs[i], cases[i].pages, opts)
+            assert torch.equal(bits(got), bits(want)), (turn, i)
+            cases[i].lens[:] = cases[i].pages.lens.cpu().tolist()
+            if turn < 2:
+                held(got, *ref.attention(cases[i], qs[i], causal=True))
+
+
+def test_a_workspace_of_any_content_and_size(device):
+    opts = Attn(causal=True)
+    for case, h in ((make(device, [2000, 900, 50], [1, 1, 2], kv_heads=2, d=64, page=16, seed=60), 4),
+                    (make(device, [3000, 20], [140, 1], kv_heads=1, d=64, page=16, seed=62), 8)):
+        q = normal((case.rows, h, 64), BF16, 1, device)
+        need = svod_amd.attention_paged_workspace(q, case.pages, opts)
+        want = svod_amd.attention_paged(q, case.pages, opts)
+        for fill in (0, 0xff, 0x7f, 1):
+            ws = torch.full((need + 256,), fill, dtype=torch.uint8, device=device)
+            assert torch.equal(bits(want), bits(svod_amd.attention_paged(q, case.pages, opts, None, ws[:need])))
+            assert bool((ws[need:] == fill).all())
+        small = svod_amd.attention_paged(q, case.pages, opts, None, ws[:need - 16])  # the keys stay whole
+        assert torch.equal(bits(small), bits(svod_amd.attention_paged(q, case.pages, Attn(causal=True, splits=1))))
+
+
+def test_left_to_the_graph(device):
+    """What a device has no kernel for, named."""
+    case = make(device, [300], [2], kv_heads=1, d=64, page=16)
+    q = normal((2, 4, 64), BF16, 1, device)
+    call = lambda p, opts, q=q, **kw: svod_amd.attention_paged(q, p, opts, **kw)
+
+    def why(f):
+        with pytest.raises(svod_amd.GraphFallback) as e:
+            f()
+        return e.value.why
+
+    some = torch.zeros(1, dtype=torch.int32, device=device)
+    for opts in (Attn(keys=KeyMask.lens(some)), Attn(bias=torch.zeros(1, 4, 2, 302, dtype=torch.float32, device=device))):
+        assert why(lambda: call(case.pages, opts)) == svod_amd.Fallback.Config
+    named = Attn(causal=True, splits=3)
+    need = svod_amd.attention_paged_workspace(q, case.pages, named)
+    lent = torch.empty(need, dtype=torch.uint8, device=device)
+    assert why(lambda: call(case.pages, named, workspace=lent[:need - 16])) == svod_amd.Fallback.Config
+    call(case.pages, named, workspace=lent)
+    shape = lambda n, page, d: Pages(*(torch.zeros(n, 1, page, d, dtype=BF16, device=device) for _ in range(2)), case.pages.table,
+                                     case.pages.lens, case.pages.starts)
+    for page, d in ((8, 64), (24, 64), (2048, 64), (16, 32), (16, 96)):
+        p, x = shape(40, page, d), torch.zeros(2, 1, d, dtype=BF16, device=device)
+        assert why(lambda: call(p, None, x)) == svod_amd.Fallback.Shape
+        assert why(lambda: svod_amd.write_pages(x, x, p)) == svod_amd.Fallback.Shape
+        assert why(lambda: svod_amd.read_pages(p, 5)) == svod_amd.Fallback.Shape
+    assert why(lambda: call(case.pages, None, normal((2, 129, 64), BF16, 1, device))) == svod_amd.Fallback.Shape
+    assert why(lambda: call(case.pages, None, q[:0])) == svod_amd.Fallback.Shape
+    with pytest.raises(svod_amd.OpError) as e:  # what is written may not be read
+        call(case.pages, None, out=q)
+    assert e.value.kind == "Launch"  # as every op answers parameters that share memory
+
+
+def test_on_the_stream_of_the_moment(device):
+    """Operands made on a stream of their own just before the calls, which follow on it."""
+    case = make(device, [900, 40], [1, 30], kv_heads=2, d=64, page=16, seed=12)
+    q0 = normal((case.rows, 4, 64), BF16, 1, device)
+    kv = normal((case.rows, 2, 64), BF16, 2, device)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        busy = torch.randn(4096, 4096, device=device)
+        for _ in range(20):
+            busy = busy @ busy * 1e-3
+        q = q0 * 2.0 + busy[0, 0].nan_to_num(0.0, 0.0, 0.0).to(BF16) * 0.0
+        svod_amd.write_pages(kv, kv, case.pages)
+        got = svod_amd.attention_paged(q, case.pages, Attn(causal=True))
+        k, _ = svod_amd.read_pages(case.pages, 901)
+    stream.synchronize()
+    for row, b, at in case.places():
+        case.k[int(case.table[b, at // 16]), :, at % 16] = kv[row].to(F64).cpu()
+        case.v[int(case.table[b, at // 16]), :, at % 16] = kv[row].to(F64).cpu()
+    held(got, *ref.attention(case, q0 * 2.0, causal=True))
+    assert torch.equal(k[0].to(F64).cpu(), case.tokens("k", 0))
