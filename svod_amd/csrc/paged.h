@@ -57,11 +57,12 @@ struct PagedParams {
   int32_t splits;        // as in PagedArgs
   int32_t slots;         // partial states there is room for
   int32_t shares;        // whether workgroups may take shares of all blocks: few rows, and tiles for more than half of the chip's places
-  // Of blocks_an_item(): the fewest blocks of an item, the workgroups that the chip holds at a time; and in us a block of a
-  // workgroup by itself and with company on its compute unit, a state of every row, and a block's bytes at the rate that memory gives.
+  // Of parts_of_all(): the fewest blocks of a part, the workgroups that the chip holds at a time, and how many times as many parts there may
+  // be; and in us a block of a workgroup by itself and with company on its compute unit, a state of every row, a block's bytes at
+  // the rate that memory gives, and a block of a workgroup among as many as there are places, when it is the last and when all are busy.
   float least;
-  int32_t places;
-  float step, crowded, states, stream;
+  int32_t places, rounds;
+  float step, crowded, states, stream, tail, even;
 };
 
 namespace {
@@ -106,6 +107,11 @@ __device__ __forceinline__ int sum_to(int x) {
 }
 
 constexpr float kStart = 5.0f, kMerge = 5.0f;  // us: from a part's place to its first block, and the merge
+// A share of all blocks: how much of the time of uneven tiles its blocks take, its own start and its two merges in us, and a tile's start in it.
+// (With PagedParams' tail and even from 98 calls of 30 to 128 sequences of 500 to 8000 keys, each whole and in shares: what is chosen is
+// 0.4 % over the better on average, 7 % at most.  Shares win where lengths differ and are long: 40 sequences of 1600 to 8000 keys, 8
+// KV heads of 128, whole 197 us, 148 in shares; of 110 to 1100 keys 28.6 and 35.)
+constexpr float kShareOf = 0.8f, kShare = 14.0f, kShareTile = 9.0f;
 // What a lane's sequence asks for: tiles of query rows, and the key blocks of one of its tiles at most.
 struct Demand {
   int start, fresh, len;  // as in Sequence
@@ -148,7 +154,9 @@ __device__ __forceinline__ int parts_of(const PagedParams &p, int blocks, const 
   return max(n, 1);
 }
 // W blocks of all tiles in parts of n are W / n + tiles parts at most.  With a tile for half of the chip's places or fewer, n is what
-// keeps all parts on places at once (a few more than there are places would wait for a whole round).  With more tiles
+// keeps all parts on places at once (a few more than there are places would wait for a whole round), or, of tiles of 128 rows, what
+// fills two rounds where that comes out ahead: parts of a tile for a third of the places or more fit one round badly (chunks of 591 and 340
+// over 17526 and 10077 keys, 32 heads over 8, 290 us in one round, 243 in two).  With more tiles
 // they are whole, but: where rows are few and the lengths differ so much or leave a last round so empty that it pays, every place
 // takes an even share of all blocks, in which a few tiles begin and end; of tiles of 128 rows, which want their sequence's
 // others beside them in the same L2 (4 chunks of 2048 over 16384 keys 964 us, 1072 in shares), only those are split that are more than
@@ -174,10 +182,12 @@ __device__ __forceinline__ Parts parts_of_all(const Deal &deal, const PagedParam
   const float most = (float)last_lane(fold_to_lane(longest, [](int a, int b) { return max(a, b); }));
   const float stream = all * p.stream;
   if (units * 2.0f <= places) {
-    const float n = __builtin_fmaxf(p.least, __builtin_ceilf(all * __builtin_amdgcn_rcpf(places - units) * (1.0f + 1e-6f)));
-    const float whole = __builtin_fmaxf(most * p.step, stream);
-    const float split = __builtin_fmaxf(n * p.crowded, stream) + kMerge + p.states * (all * __builtin_amdgcn_rcpf(n * units) + 1.0f);
-    if (n < most && split < whole) parts.most = (int)n;
+    float best = __builtin_fmaxf(most * p.step, stream);
+    for (int round = 1; round <= p.rounds; round++) {
+      const float n = __builtin_fmaxf(p.least, __builtin_ceilf(all * __builtin_amdgcn_rcpf(places * (float)round - units) * (1.0f + 1e-6f)));
+      const float split = __builtin_fmaxf(n * (float)round * p.crowded, stream) + kMerge + p.states * (all * __builtin_amdgcn_rcpf(n * units) + 1.0f);
+      if (n < most && split < best) best = split, parts.most = (int)n;
+    }
   } else if (!SHARES) {
     const float n = __builtin_fmaxf(p.least, __builtin_ceilf(2.0f * all * a_place * (1.0f + 1e-6f)));
     const float rest = all * a_place * p.crowded;
@@ -185,9 +195,9 @@ __device__ __forceinline__ Parts parts_of_all(const Deal &deal, const PagedParam
       parts.most = (int)n;
   } else if constexpr (SHARES) {
     const int share = p.places / deal.kv_heads > 0 ? (blocks + p.places / deal.kv_heads - 1) / (p.places / deal.kv_heads) : blocks;
-    const float rounds = __builtin_ceilf(units * a_place);
-    const float whole = __builtin_fmaxf(most, rounds * all * __builtin_amdgcn_rcpf(units)) * p.crowded;
-    const float shared = all * a_place * p.crowded + kStart * units * a_place + kMerge + p.states;
+    const float even = all * a_place * p.even;
+    const float whole = kStart * __builtin_ceilf(units * a_place) + __builtin_fmaxf(most * p.tail, even);
+    const float shared = kShareOf * even + kShare + kShareTile * units * a_place;
     if (p.slots > 0 && share > 1 && shared < whole) parts.run = share;
   }
   return parts;
@@ -258,22 +268,25 @@ __device__ __forceinline__ Place place_of(const Deal &deal, const PagedParams &p
 // What a workgroup does: parts [at, to) of a KV head.  The KV heads of a part are neighbours in the launch, their pages are
 // neighbours in memory.
 struct Turn {
-  int kvh, mine, at, to;
+  int kvh, mine, at;
   Parts parts;
   Demand first;
+  __device__ __forceinline__ void whose(const Deal &deal) {
+    const uint32_t wg = __builtin_amdgcn_workgroup_id_x();
+    mine = (int)over(wg, (uint32_t)deal.kv_heads, deal.kvh_rcp);
+    kvh = (int)(wg - (uint32_t)mine * (uint32_t)deal.kv_heads);
+  }
+  __device__ __forceinline__ int to() const { return mine * parts.run + parts.run; }
 };
 template <bool SHARES>
 __device__ __forceinline__ Turn turn_of(const Deal &deal, const PagedParams &p) {
-  const uint32_t wg = __builtin_amdgcn_workgroup_id_x();
   Turn t;
-  t.mine = (int)over(wg, (uint32_t)deal.kv_heads, deal.kvh_rcp);
-  t.kvh = (int)(wg - (uint32_t)t.mine * (uint32_t)deal.kv_heads);
+  t.whose(deal);
   t.first = demand_of(deal, lane_id());
   t.parts = parts_of_all<SHARES>(deal, p, t.first);
   t.at = t.mine * t.parts.run;
-  t.to = t.at + t.parts.run;
   // The merge's kernel goes by the same deal: it is told what this launch went by.
-  if (p.told != nullptr && wg == 0 && __builtin_amdgcn_workitem_id_x() == 0) p.told[0] = t.parts.most, p.told[1] = t.parts.run;
+  if (p.told != nullptr && __builtin_amdgcn_workgroup_id_x() == 0 && __builtin_amdgcn_workitem_id_x() == 0) p.told[0] = t.parts.most, p.told[1] = t.parts.run;
   return t;
 }
 // The workgroups that have a tile of several parts: one a part, or those in whose shares it lies; and the slots of their partial
@@ -316,7 +329,7 @@ __device__ __forceinline__ Work work_of(const Deal &deal, const PagedParams &p, 
   w.kvh = t.kvh;
   w.at = place_of<false, CHUNKS>(deal, p, t.at, t.first, t.parts);
   if (!w.at.found) return w;
-  w.taken = SHARES ? min(w.at.parts - w.at.part, t.to - t.at) : 1;
+  w.taken = SHARES ? min(w.at.parts - w.at.part, t.to() - t.at) : 1;
   w.whole = w.taken == w.at.parts;
   w.some = true;
   if (!w.whole) {

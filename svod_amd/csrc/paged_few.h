@@ -62,12 +62,12 @@ struct Few {
   static constexpr int kStateRow = (D + 4) * 4;
   static constexpr int kState = kRows * kStateRow + kRows * 8;
   static constexpr int kWaveLds = kTile > kState ? kTile : kState;
-  static constexpr int kLds = kWaves * kWaveLds;  // and a word behind
+  static constexpr int kLds = kWaves * kWaveLds;  // and behind it a word, and 16 bytes a wave
   // A state in memory: the rows' columns, then their maxima and sums.
   static constexpr int kStateBytes = kRows * (D + 2) * 4;
   // Waves a SIMD, which are workgroups a compute unit: by registers and LDS.
   static constexpr int kResident = D == 256 || (D == 128 && RT == 2) ? 1 : (D == 128 || RT == 2) ? 2 : 3;
-  static_assert(kResident * (kLds + 16) <= 160 * 1024, "the workgroups' LDS");
+  static_assert(kResident * (kLds + 16 * (1 + kWaves)) <= 160 * 1024, "the workgroups' LDS");
 };
 // A tile of V is read by 16 lanes as 4 rows of 32 bytes, 8 rows to half a wave: the 32-byte groups of a row are xor-ed with what
 // tells 8 rows apart within the period of the banks (256 bytes: a row of 128 values, half of one of 256, two of 64).

@@ -15,26 +15,59 @@
 namespace svodk {
 namespace {
 
+// The parameters as a turn reads them: from the launch's arguments, and not known to be what the turn before had.  (What a
+// loop of turns keeps of them in registers is more than there are: 16-bit pools at D 128 spilled, and 128 sequences of 300 to 3000 keys, 8
+// KV heads, took 185 us where it is 169.)
+struct Arguments {
+  uint64_t deal_lens, deal_starts;
+  uint32_t deal_batch, deal_wide, deal_limit, deal_rows, deal_tokens, deal_tokens_rcp, deal_window_blocks, deal_kv_heads, deal_kvh_rcp;
+  PagedParams p;
+  __device__ Deal deal() const { return SVODK_DEAL; }
+};
+__device__ __forceinline__ Arguments arguments_of_turn() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef const __attribute__((address_space(4))) Arguments *At;
+  At at = (At)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *at;
+#else
+  return Arguments{};
+#endif
+}
+
 template <int D, int RT, bool F16, bool CODED, bool SHARES>
 __global__ __launch_bounds__(few::kWaves * 64, (few::Few<D, RT>::kResident)) void paged_few_kernel(SVODK_DEAL_PARAMS, PagedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const Deal deal = SVODK_DEAL;
-  Turn turn = turn_of<SHARES>(deal, p);
-  do {
-    const Work work = work_of<SHARES, false>(deal, p, turn);
-    if (!work.at.found) return;
+  if constexpr (SHARES) {
+    // What a wave carries from turn to turn lies behind its workgroup's LDS.
+    auto kept_at = [&]() { return reinterpret_cast<volatile int *>(smem + few::Few<D, RT>::kLds + 16 + 16 * uniform((int)__builtin_amdgcn_workitem_id_x() >> 6)); };
+    Turn turn = turn_of<true>(deal, p);
+    kept_at()[1] = turn.parts.most, kept_at()[2] = turn.parts.run;
+    do {
+      const Arguments here = arguments_of_turn();
+      const Work work = work_of<true, false>(here.deal(), here.p, turn);
+      if (!work.at.found) return;
+      kept_at()[0] = turn.at + work.taken < turn.to() ? turn.at + work.taken : -1;
+      if (work.some) few::item<D, RT, F16, CODED, true>(smem, here.deal(), here.p, work);
+      __syncthreads();  // the states have been read
+      volatile int *const kept = kept_at();
+      turn.at = uniform(kept[0]), turn.parts.most = uniform(kept[1]), turn.parts.run = uniform(kept[2]);
+      const Deal again = arguments_of_turn().deal();
+      turn.whose(again);
+      turn.first = demand_of(again, lane_of_turn());
+    } while (turn.at >= 0);
+  } else {
+    const Work work = work_of<false, false>(deal, p, turn_of<false>(deal, p));
     if (work.some) few::item<D, RT, F16, CODED, true>(smem, deal, p, work);
-    if (SHARES) __syncthreads();  // the states have been read
-    turn.at += work.taken;
-    if (SHARES) turn.first = demand_of(deal, lane_of_turn());  // asked for again: held in registers it would cost the loop five
-  } while (SHARES && turn.at < turn.to);
+  }
 #endif
 }
 
 template <int D, int RT, bool F16, bool CODED>
 hipError_t launch(const PagedLaunch &l, hipStream_t stream) {
-  constexpr int kLds = few::Few<D, RT>::kLds + 16;
+  constexpr int kLds = few::Few<D, RT>::kLds + 16 * (1 + few::kWaves);
   if (l.p.shares)
     return Launch<paged_few_kernel<D, RT, F16, CODED, true>>::run(l.grid, few::kWaves * 64, kLds, kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);
   return Launch<paged_few_kernel<D, RT, F16, CODED, false>>::run(l.grid, few::kWaves * 64, kLds, kLds, stream, SVODK_DEAL_ARGS(l.deal), l.p);

@@ -534,6 +534,10 @@ int resident(const PagedArgs &a) {
 int64_t places(const PagedArgs &a) { return (int64_t)kPagedUnits * resident(a); }
 // Whether there may be tiles for more than half of the chip's places.
 bool dense(const PagedArgs &a) { return 2 * tiles_at_most(a) * a.pages.kv_heads > places(a); }
+// Rounds of places that parts may take: two where tiles of 128 rows may be for a quarter of the places and more (parts_of_all).
+int rounds(const PagedArgs &a) {
+  return paged_tile_rows(a) == 128 && !dense(a) && 4 * tiles_at_most(a) * a.pages.kv_heads >= places(a) ? 2 : 1;
+}
 int64_t blocks_at_most(const PagedArgs &a) { return (((int64_t)a.pages.columns << a.pages.page_log2) + kBkv - 1) / kBkv; }
 }  // namespace
 
@@ -552,7 +556,7 @@ int64_t paged_slots(const PagedArgs &a) {
   // Too short to be worth a merge, whatever the lengths; and blocks of all tiles are counted in 31 bits.
   // (A state for each of many tiles of 128 rows would be gigabytes, where none is more than a small part of the launch.)
   if (!few && tiles > 4 * places(a)) return 0;
-  if (blocks <= (few ? 8 : 4) || tiles / a.pages.kv_heads * blocks > 0x3fffffff || (dense(a) && blocks < (few ? 16 : 64))) return 0;
+  if (blocks <= (few ? 8 : 4) || tiles / a.pages.kv_heads * blocks > 0x3fffffff || (dense(a) && blocks < (few ? 32 : 64))) return 0;
   return few && dense(a) ? 2 * (places(a) + a.pages.kv_heads) : paged_workgroups(a);
 }
 
@@ -560,7 +564,7 @@ int64_t paged_slots(const PagedArgs &a) {
 // where long ones alone are (parts_of_all).  (With one for every partial state that there might be 16 sequences over 210 to 2100
 // keys took 32.8 us: one without a part costs a place the deal.)
 int64_t paged_workgroups(const PagedArgs &a) {
-  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, round = a.pages.kv_heads, p = (places(a) + round) / round * round;
+  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, round = a.pages.kv_heads, p = (places(a) * rounds(a) + round) / round * round;
   if (a.splits > 1) return tiles * a.splits;
   if (a.splits == 1) return tiles;
   if (dense(a) && paged_tile_rows(a) == 128) return tiles + (places(a) / 2 + round) / round * round;
@@ -608,8 +612,9 @@ PagedLaunch paged_launch(const PagedArgs &a) {
   p.splits = a.splits;
   p.slots = (int32_t)slots;
   p.shares = few && slots > 0 && a.splits == 0 && dense(a);
-  p.least = few ? 4.0f : 2.0f, p.places = (int32_t)places(a);
-  p.step = few ? 0.6f : 1.4f, p.crowded = !few ? 1.75f : dense(a) ? 1.0f : 0.6f;
+  p.least = few ? 4.0f : 2.0f, p.places = (int32_t)places(a), p.rounds = rounds(a);
+  p.step = few ? 0.6f : 1.4f, p.crowded = few ? 0.6f : 1.75f;
+  p.tail = g.k_scale ? 0.85f : 1.35f, p.even = (g.k_scale ? 1.65f : 2.3f) * (g.d == 256 ? 1.4f : 1.0f);
   // A state is written and read at 5 MB a us: of every row, or of two tiles a place.
   const double of_rows = (double)g.rows * a.heads, of_places = 2.0 * places(a) * rows;
   p.states = (float)((p.shares && of_places < of_rows ? of_places : of_rows) * (g.d + 2) * 8 / 5e6);
