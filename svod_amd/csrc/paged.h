@@ -60,8 +60,8 @@ struct PagedParams {
   // Of parts_of_all(): the fewest blocks of a part, the workgroups that the chip holds at a time, and how many times as many parts there may
   // be; and in us a block of a workgroup by itself and with company on its compute unit, a state of every row, a block's bytes at
   // the rate that memory gives, and a block of a workgroup among as many as there are places, when it is the last and when all are busy.
-  float least;
-  int32_t places, rounds;
+  float least, turn;  // turn: 1 over the blocks that a workgroup takes at a time
+  int32_t places, spread, rounds;  // spread: of the places, those that parts go to where there are tiles for a quarter of them or fewer
   float step, crowded, states, stream, tail, even;
 };
 
@@ -154,7 +154,8 @@ __device__ __forceinline__ int parts_of(const PagedParams &p, int blocks, const 
   return max(n, 1);
 }
 // W blocks of all tiles in parts of n are W / n + tiles parts at most.  With a tile for half of the chip's places or fewer, n is what
-// keeps all parts on places at once (a few more than there are places would wait for a whole round), or, of tiles of 128 rows, what
+// keeps all parts on places at once (a few more than there are places would wait for a whole round; and as many fewer leave compute units
+// with one where others have two: 2 sequences of 4700 keys, 8 KV heads of 128, in 192 parts 16.6 us, 320 18.2, 512 16.9), or, of tiles of 128 rows, what
 // fills two rounds where that comes out ahead: parts of a tile for a third of the places or more fit one round badly (chunks of 591 and 340
 // over 17526 and 10077 keys, 32 heads over 8, 290 us in one round, 243 in two).  With more tiles
 // they are whole, but: where rows are few and the lengths differ so much or leave a last round so empty that it pays, every place
@@ -182,9 +183,30 @@ __device__ __forceinline__ Parts parts_of_all(const Deal &deal, const PagedParam
   const float most = (float)last_lane(fold_to_lane(longest, [](int a, int b) { return max(a, b); }));
   const float stream = all * p.stream;
   if (units * 2.0f <= places) {
+    const float spread = units * 4.0f <= (float)p.spread ? (float)p.spread : places;
     float best = __builtin_fmaxf(most * p.step, stream);
     for (int round = 1; round <= p.rounds; round++) {
-      const float n = __builtin_fmaxf(p.least, __builtin_ceilf(all * __builtin_amdgcn_rcpf(places * (float)round - units) * (1.0f + 1e-6f)));
+      // What keeps the parts to the places whatever the lengths: a part a tile too many; fewer where the lengths go up, or where with half a part
+      // a tile too many the longest take fewer turns.
+      const float all_places = spread * (float)round;
+      auto fewest = [&](float slack) {
+        return __builtin_fmaxf(p.least, __builtin_ceilf(all * __builtin_amdgcn_rcpf(all_places - slack * units) * (1.0f + 1e-6f)));
+      };
+      auto fit = [&](float n) {
+        const Parts tried = {(int)n, 1};
+        int count = 0;
+        for (int base = 0; base < deal.batch; base += 64) {
+          const Demand d = base == 0 ? first : demand_of(deal, base + lane);
+          count += d.tiles * parts_of(p, d.blocks, tried);
+        }
+        return heads * (float)last_lane(sum_to(count)) <= all_places;
+      };
+      float n = fewest(1.0f);
+      const float tight = fewest(0.0f), half = fewest(0.5f);
+      if (fit(tight))
+        n = tight;
+      else if (__builtin_ceilf(half * p.turn) < __builtin_ceilf(n * p.turn) && fit(half))
+        n = half;
       const float split = __builtin_fmaxf(n * (float)round * p.crowded, stream) + kMerge + p.states * (all * __builtin_amdgcn_rcpf(n * units) + 1.0f);
       if (n < most && split < best) best = split, parts.most = (int)n;
     }

@@ -534,6 +534,9 @@ int resident(const PagedArgs &a) {
 int64_t places(const PagedArgs &a) { return (int64_t)kPagedUnits * resident(a); }
 // Whether there may be tiles for more than half of the chip's places.
 bool dense(const PagedArgs &a) { return 2 * tiles_at_most(a) * a.pages.kv_heads > places(a); }
+// The places that parts go to where there are tiles for a quarter of them or fewer: of few rows over 16 bits one workgroup a compute unit,
+// which take what the memory gives; codes want the second one's waves beside them.
+int64_t spread(const PagedArgs &a) { return paged_tile_rows(a) != 128 && a.pages.k_scale == nullptr ? kPagedUnits : places(a); }
 // Rounds of places that parts may take: two where tiles of 128 rows may be for a quarter of the places and more (parts_of_all).
 int rounds(const PagedArgs &a) {
   return paged_tile_rows(a) == 128 && !dense(a) && 4 * tiles_at_most(a) * a.pages.kv_heads >= places(a) ? 2 : 1;
@@ -564,7 +567,7 @@ int64_t paged_slots(const PagedArgs &a) {
 // where long ones alone are (parts_of_all).  (With one for every partial state that there might be 16 sequences over 210 to 2100
 // keys took 32.8 us: one without a part costs a place the deal.)
 int64_t paged_workgroups(const PagedArgs &a) {
-  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, round = a.pages.kv_heads, p = (places(a) * rounds(a) + round) / round * round;
+  const int64_t tiles = tiles_at_most(a) * a.pages.kv_heads, round = a.pages.kv_heads, p = ((4 * tiles <= spread(a) ? spread(a) : places(a)) * rounds(a) + round) / round * round;
   if (a.splits > 1) return tiles * a.splits;
   if (a.splits == 1) return tiles;
   if (dense(a) && paged_tile_rows(a) == 128) return tiles + (places(a) / 2 + round) / round * round;
@@ -612,8 +615,8 @@ PagedLaunch paged_launch(const PagedArgs &a) {
   p.splits = a.splits;
   p.slots = (int32_t)slots;
   p.shares = few && slots > 0 && a.splits == 0 && dense(a);
-  p.least = few ? 4.0f : 2.0f, p.places = (int32_t)places(a), p.rounds = rounds(a);
-  p.step = few ? 0.6f : 1.4f, p.crowded = few ? 0.6f : 1.75f;
+  p.least = few ? 4.0f : 2.0f, p.turn = few ? 0.25f : 1.0f, p.places = (int32_t)places(a), p.spread = (int32_t)spread(a), p.rounds = rounds(a);
+  p.step = !few ? 1.4f : (g.k_scale ? 0.68f : 0.95f) * g.d / 128, p.crowded = few ? p.step : 1.75f;
   p.tail = g.k_scale ? 0.85f : 1.35f, p.even = (g.k_scale ? 1.65f : 2.3f) * (g.d == 256 ? 1.4f : 1.0f);
   // A state is written and read at 5 MB a us: of every row, or of two tiles a place.
   const double of_rows = (double)g.rows * a.heads, of_places = 2.0 * places(a) * rows;
