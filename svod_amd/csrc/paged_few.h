@@ -75,11 +75,6 @@ template <int D>
 __device__ __forceinline__ constexpr int turn_of(int row) {
   return D == 64 ? (row >> 1) & 3 : row & 7;
 }
-// And it is written, of codes, in pieces of 16 bytes 32 apart: what lies a period of the banks on has its 16-byte halves the other way round.
-template <int D>
-__device__ __forceinline__ constexpr int half_of(int row, int group) {
-  return (D == 64 ? row >> 1 : D == 128 ? row : group >> 3) & 1;
-}
 
 // x folded over the four lanes that share a query row (l % 16).
 template <typename Op>
@@ -241,12 +236,12 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
   for (int i = 0; i < kVPer; i++) {
     const int row = i * kVRows + lane / kVLanes, piece = lane % kVLanes;  // a piece: 8 values, or 16 codes
     const int group = CODED ? piece : piece >> 1;
-    v_put[i] = row * L::kRowBytes + ((group ^ turn_of<D>(row)) << 5) + (((CODED ? 0 : piece & 1) ^ half_of<D>(row, group)) << 4);
+    v_put[i] = row * L::kRowBytes + ((group ^ turn_of<D>(row)) << 5) + (CODED ? 0 : (piece & 1) << 4);
   }
 #pragma unroll
   for (int db = 0; db < DB; db++) {
     const int row = 4 * lq + (lr >> 2);
-    v_get[db] = row * L::kRowBytes + ((db ^ turn_of<D>(row)) << 5) + (((lane & 3) << 3) ^ (half_of<D>(row, db) << 4));
+    v_get[db] = row * L::kRowBytes + ((db ^ turn_of<D>(row)) << 5) + ((lane & 3) << 3);
   }
 
   const bool positive = p.scale > 0.0f;
@@ -341,7 +336,7 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
           const float scale = scale_of(v_scale[r][i]);
           *reinterpret_cast<u32x4 *>(to) = u32x4{widen_codes<F16, false>(c[0], scale), widen_codes<F16, true>(c[0], scale),
                                                  widen_codes<F16, false>(c[1], scale), widen_codes<F16, true>(c[1], scale)};
-          *reinterpret_cast<u32x4 *>(tile + ((16 * r * L::kRowBytes + v_put[i]) ^ 16)) = u32x4{widen_codes<F16, false>(c[2], scale), widen_codes<F16, true>(c[2], scale),
+          *reinterpret_cast<u32x4 *>(to + 16) = u32x4{widen_codes<F16, false>(c[2], scale), widen_codes<F16, true>(c[2], scale),
                                                       widen_codes<F16, false>(c[3], scale), widen_codes<F16, true>(c[3], scale)};
         } else {
           *reinterpret_cast<u32x4 *>(to) = c;
