@@ -379,6 +379,7 @@ template <int D, int NW, bool F16, bool CODED>
 __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void paged_kernel(SVODK_DEAL_PARAMS, PagedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  static_assert(few::Few<D, 1>::kLds <= Tile<D>::kLds, "both forms' LDS");
   const Deal deal = SVODK_DEAL;
   const Work work = work_of<false, true>(deal, p, turn_of<false>(deal, p));
   if (!work.some) return;

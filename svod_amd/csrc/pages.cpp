@@ -160,8 +160,8 @@ int take_paged(const svodk_tensor *q, const svodk_pages *pages, const svodk_attn
   const int64_t blocks = (far + 63) / 64;
   a.splits = opts->splits <= 0 ? 0 : (int32_t)std::min<int64_t>(opts->splits, blocks);
   if (svodk::paged_slots(a) == 0) a.splits = 1;
-  // A launch's workgroups are counted in 31 bits, and so are its partial states.
-  if (svodk::paged_workgroups(a) > 0x7fffffff) why = SVODK_GRAPH_SHAPE;
+  // A launch's threads are counted in 32 bits, 256 a workgroup.
+  if (svodk::paged_workgroups(a) > 0xffffff) why = SVODK_GRAPH_SHAPE;
   // And the bytes of the states of a named count of splits in 32.
   if (a.splits > 1 && svodk::paged_workspace(a) > 0x7fffffff) why = SVODK_GRAPH_CONFIG;
   return 0;

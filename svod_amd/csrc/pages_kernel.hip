@@ -213,7 +213,7 @@ template <int D, bool F16, bool CODED, int HEADS>
 hipError_t write_heads(const PagesArgs &a, const void *k, const void *v, hipStream_t stream) {
   const int64_t groups = ((int64_t)a.rows * D / 8 + 63) / 64, strips = (a.kv_heads + HEADS - 1) / HEADS;
   const int64_t grid = (groups * strips + kWaves - 1) / kWaves;
-  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
+  if (grid > 0xffffffff / (kWaves * 64)) return hipErrorInvalidConfiguration;  // a launch's threads are counted in 32 bits
   return Launch<write_pages_kernel<D, F16, CODED, HEADS>>::run(grid, kWaves * 64, 0, 0, stream, a, (uint32_t)strips, (const uint16_t *)k,
                                                                (const uint16_t *)v);
 }
@@ -226,7 +226,7 @@ hipError_t write(const PagesArgs &a, const void *k, const void *v, hipStream_t s
 template <int D, bool F16, bool CODED>
 hipError_t read(const PagesArgs &a, int32_t tokens, void *k, void *v, hipStream_t stream) {
   const int64_t groups = ((int64_t)tokens * D / 8 + 63) / 64, waves = groups * a.batch * a.kv_heads, grid = (waves + kWaves - 1) / kWaves;
-  if (grid > 0x7fffffff / kWaves) return hipErrorInvalidConfiguration;
+  if (grid > 0xffffffff / (kWaves * 64)) return hipErrorInvalidConfiguration;  // a launch's threads are counted in 32 bits
   return Launch<read_pages_kernel<D, F16, CODED>>::run(grid, kWaves * 64, 0, 0, stream, a, tokens, (uint32_t)groups, (uint16_t *)k, (uint16_t *)v);
 }
 
