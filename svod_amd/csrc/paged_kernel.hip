@@ -15,6 +15,8 @@
 // in f32; merge_kernel adds them up, so a call's result depends on nothing but its inputs.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "kernels.h"
 #include "launch.h"
 
@@ -542,7 +544,14 @@ int64_t spread(const PagedArgs &a) { return paged_tile_rows(a) != 128 && a.pages
 int rounds(const PagedArgs &a) {
   return paged_tile_rows(a) == 128 && !dense(a) && 4 * tiles_at_most(a) * a.pages.kv_heads >= places(a) ? 2 : 1;
 }
-int64_t blocks_at_most(const PagedArgs &a) { return (((int64_t)a.pages.columns << a.pages.page_log2) + kBkv - 1) / kBkv; }
+// Key blocks that a window leaves a tile.
+int64_t window_blocks(const PagedArgs &a) {
+  const int64_t tokens = paged_tile_rows(a) / (a.heads / a.pages.kv_heads);
+  return a.win_left < 0 ? 0x7fffffff : std::min<int64_t>(((int64_t)a.win_left + a.win_right + tokens) / kBkv + 2, 0x7fffffff);
+}
+int64_t blocks_at_most(const PagedArgs &a) {
+  return std::min((((int64_t)a.pages.columns << a.pages.page_log2) + kBkv - 1) / kBkv, window_blocks(a));
+}
 }  // namespace
 
 int paged_tile_rows(const PagedArgs &a) {
@@ -557,10 +566,12 @@ int64_t paged_slots(const PagedArgs &a) {
   if (a.splits == 1 || blocks <= 1) return 0;
   if (a.splits > 1) return tiles * a.splits;
   const bool few = paged_tile_rows(a) != 128;
-  // Too short to be worth a merge, whatever the lengths; and blocks of all tiles are counted in 31 bits.
-  // (A state for each of many tiles of 128 rows would be gigabytes, where none is more than a small part of the launch.)
+  // A state for each of many tiles of 128 rows would be gigabytes, where none is more than a small part of the launch.
   if (!few && tiles > 4 * places(a)) return 0;
-  if (blocks <= (few ? 8 : 4) || tiles / a.pages.kv_heads * blocks > 0x3fffffff || (dense(a) && blocks < (few ? 32 : 64))) return 0;
+  // Too short to be worth a merge, whatever the lengths: for tiles of 128 rows it is a launch (two chunks of 1001 in a window of 1024, 256
+  // tiles, 34.9 us with it and 32.1 without, nothing split in either).  And blocks of all tiles are counted in 31 bits.
+  const int64_t least = few ? (dense(a) ? 32 : 9) : dense(a) ? 64 : rounds(a) > 1 ? 24 : 5;
+  if (blocks < least || tiles / a.pages.kv_heads * blocks > 0x3fffffff) return 0;
   return few && dense(a) ? 2 * (places(a) + a.pages.kv_heads) : paged_workgroups(a);
 }
 
@@ -592,11 +603,7 @@ PagedLaunch paged_launch(const PagedArgs &a) {
   d.lens = g.lens, d.starts = g.starts, d.batch = g.batch, d.wide = (g.lens_i64 ? 1 : 0) | (g.starts_i64 ? 2 : 0);
   d.limit = g.columns << g.page_log2, d.rows = g.rows;
   d.tokens = rows / group, d.tokens_rcp = rcp_of(d.tokens);
-  d.window_blocks = 0x7fffffff;
-  if (a.win_left >= 0) {
-    const int64_t w = ((int64_t)a.win_left + a.win_right + d.tokens) / kBkv + 2;
-    d.window_blocks = (int)(w < 0x7fffffff ? w : 0x7fffffff);
-  }
+  d.window_blocks = (int32_t)window_blocks(a);
   d.kv_heads = g.kv_heads, d.kvh_rcp = rcp_of(g.kv_heads);
   PagedParams &p = l.p;
   p.q = (const uint16_t *)a.q, p.o = (uint16_t *)a.o;
