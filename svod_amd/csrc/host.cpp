@@ -610,17 +610,28 @@ struct PagesCall {
 
   explicit PagesCall(PyObject *pages) {
     pool = kept(get(pages, names.k));
-    describe(pool, k, pool_dtype_of), describe(kept(get(pages, names.v)), v, pool_dtype_of);
+    take(pool, k, pool_dtype_of), take(kept(get(pages, names.v)), v, pool_dtype_of);
     p.k = &k, p.v = &v;
-    describe(kept(get(pages, names.table)), table), describe(kept(get(pages, names.lens)), lens);
+    take(kept(get(pages, names.table)), table), take(kept(get(pages, names.lens)), lens);
     p.table = &table, p.lens = &lens;
-    p.starts = maybe_attr(kept, pages, names.starts, starts);
+    PyObject *const from = kept(get(pages, names.starts));
+    if (from != Py_None) take(from, starts), p.starts = &starts;
     Ref scales(get(pages, names.scales));
     if (scales != Py_None) {
-      describe(kept(PySequence_GetItem(scales, 0)), k_scale, pool_dtype_of);
-      describe(kept(PySequence_GetItem(scales, 1)), v_scale, pool_dtype_of);
+      take(kept(PySequence_GetItem(scales, 0)), k_scale, pool_dtype_of);
+      take(kept(PySequence_GetItem(scales, 1)), v_scale, pool_dtype_of);
       p.k_scale = &k_scale, p.v_scale = &v_scale;
     }
+  }
+  // An operand of the call, which has to be where the pool is: lengths and tables are easily kept on the host, whose addresses a kernel
+  // must not follow.  With all of them there the op words what it finds first; it runs nothing over null.
+  void take(PyObject *o, svodk_tensor &d, int (*type_of)(at::ScalarType) = dtype_of) const {
+    describe(o, d, type_of);
+    beside(tensor(o));
+    if (!tensor(o).is_cuda() && c10::hip::device_count() > 0) d.data = nullptr;
+  }
+  void beside(const at::Tensor &t) const {
+    if (t.device() != tensor(pool).device()) op_failed("Argument", "the operands and the pages are on more than one device");
   }
 };
 
@@ -630,7 +641,7 @@ PyObject *py_write_pages(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   SVODK_BEGIN
   PagesCall call(args[2]);
   svodk_tensor kd, vd;
-  describe(args[0], kd), describe(args[1], vd);
+  call.take(args[0], kd), call.take(args[1], vd);
   void *stream = stream_of(tensor(args[0]));
   const int status = unlocked(tensor(args[0]), [&] { return pages_abi.write_pages(&kd, &vd, &call.p, stream); });
   Ref none(held(Py_None));
@@ -669,7 +680,7 @@ PyObject *py_read_pages(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   Ref out(made);
   svodk_tensor kd, vd;
   Kept kept;
-  describe(kept(PySequence_GetItem(out, 0)), kd), describe(kept(PySequence_GetItem(out, 1)), vd);
+  call.take(kept(PySequence_GetItem(out, 0)), kd), call.take(kept(PySequence_GetItem(out, 1)), vd);
   void *stream = stream_of(tensor(call.pool));
   const int status = unlocked(tensor(call.pool), [&] { return pages_abi.read_pages(&call.p, &kd, &vd, stream); });
   return answer("read_pages", status, out);
@@ -685,7 +696,7 @@ PyObject *py_attention_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs
   PagesCall pages(args[1]);
   AttnCall call(args[2]);
   svodk_tensor qd, od;
-  describe(q, qd), describe(out, od);
+  pages.take(q, qd), pages.take(out, od);
   Ref lent(held(args[4]));
   if (lent == Py_None && call.a.splits != 1) {
     const int64_t need = pages_abi.attention_paged_workspace(&qd, &pages.p, &call.a);
@@ -693,6 +704,8 @@ PyObject *py_attention_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs
   }
   if (lent != Py_None) {
     const at::Tensor &t = tensor(lent);
+    pages.beside(t);
+    if (!t.is_contiguous()) op_failed("Argument", "attention_paged: a workspace that is not dense");
     call.a.workspace = t.data_ptr(), call.a.workspace_bytes = (int64_t)t.numel() * (int64_t)t.element_size();
   }
   void *stream = stream_of(tensor(q));

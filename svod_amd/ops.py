@@ -370,7 +370,8 @@ class Pages:
     Sequence b has ``lens[b]`` tokens, its token at position p in row ``p % page`` of page ``table[b, p // page]`` (int32, entries
     past its pages unused).  The last ``starts[b + 1] - starts[b]`` of them are the step's new ones, rows ``starts[b]`` and on of
     the step's packed operands.  ``lens`` and ``starts`` are int32 or int64.  What they hold is looked at on the device alone:
-    one object, and one captured graph, serve every step whose operands have as many rows."""
+    one object, and one captured graph, serve every step whose operands have as many rows.  All of it is on the operands' device:
+    lengths or a table on the host are refused."""
 
     k: torch.Tensor
     v: torch.Tensor

@@ -618,6 +618,35 @@ def test_left_to_the_graph(device):
     assert e.value.kind == "Launch"  # as every op answers parameters that share memory
 
 
+def test_operands_that_the_host_holds_are_refused(device):
+    """Lengths, starts and tables are easily kept on the host: no kernel follows an address there."""
+    case = make(device, [300, 40], [2, 1], kv_heads=1, d=64, page=16, coded=True)
+    q, k = normal((3, 4, 64), BF16, 1, device), normal((3, 1, 64), BF16, 2, device)
+    fields = case.pages.__dict__
+
+    def refused(f):
+        with pytest.raises(svod_amd.OpError) as e:
+            f()
+        assert e.value.kind == "Argument", e.value
+
+    moved = [Pages(**{**fields, n: fields[n].cpu()}) for n in ("k", "v", "table", "lens", "starts")]
+    moved.append(Pages(**{**fields, "scales": (fields["scales"][0], fields["scales"][1].cpu())}))
+    for p in moved:
+        refused(lambda: svod_amd.attention_paged(q, p, Attn(causal=True)))
+        refused(lambda: svod_amd.write_pages(k, k, p))
+        refused(lambda: svod_amd.read_pages(p, 7))
+    refused(lambda: svod_amd.attention_paged(q.cpu(), case.pages))
+    refused(lambda: svod_amd.attention_paged(q, case.pages, out=torch.empty(3, 4, 64, dtype=BF16)))
+    refused(lambda: svod_amd.attention_paged(q, case.pages, workspace=torch.empty(1 << 20, dtype=torch.uint8)))
+    refused(lambda: svod_amd.write_pages(k, k.cpu(), case.pages))
+    everything = Pages(**{n: (tuple(y.cpu() for y in x) if n == "scales" else x.cpu()) for n, x in fields.items()})
+    refused(lambda: svod_amd.attention_paged(q.cpu(), everything))
+    refused(lambda: svod_amd.write_pages(k.cpu(), k.cpu(), everything))
+    refused(lambda: svod_amd.read_pages(everything, 7))
+    lent = torch.empty(2, 1 << 20, dtype=torch.uint8, device=device)
+    refused(lambda: svod_amd.attention_paged(q, case.pages, workspace=lent[:, ::2]))
+
+
 def test_on_the_stream_of_the_moment(device):
     """Operands made on a stream of their own just before the calls, which follow on it."""
     case = make(device, [900, 40], [1, 30], kv_heads=2, d=64, page=16, seed=12)
