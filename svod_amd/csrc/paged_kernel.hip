@@ -12,7 +12,8 @@
 // The key loop here is the attention kernel's (attention_step.h): 64 keys a step through an LDS ring, both products transposed
 // on v_mfma_f32_32x32x16 so that a query is a lane, scores, maximum and sum in 32 bits, p rounded to 16 bits for the
 // second product.  What is this file's own is how keys come into the ring.  A split leaves its accumulator, maximum and sum
-// in f32; merge_kernel adds them up, so a call's result depends on nothing but its inputs.
+// in f32; merge_kernel adds them up, so a call's result depends on nothing but its inputs.  (4 chunks of 2048 over 12288 to 16384 keys, 16 heads
+// over 8 of 128: 960 us, 994 TFLOP/s, over codes 1060; two chunks of 1001 beside 30 tokens, in codes, in a window of 1024: 41 us.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

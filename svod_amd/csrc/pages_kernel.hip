@@ -171,7 +171,8 @@ __global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, u
 #endif
 }
 
-// ---- and out of them.  A wave takes 64 / LANES neighbouring positions of one (sequence, KV head): no page ends inside.
+// ---- and out of them.  A wave takes 64 / LANES neighbouring positions of one (sequence, KV head): no page ends inside.  (32768 rows of 8
+// heads of 128 in codes, 202 MB: 33 us by itself, 6.1 TB/s; bound by memory.)
 template <int D, bool F16, bool CODED>
 __global__ __launch_bounds__(kWaves * 64) void read_pages_kernel(PagesArgs p, int tokens, uint32_t groups, uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
 #if defined(__HIP_DEVICE_COMPILE__)
