@@ -668,3 +668,51 @@ def test_on_the_stream_of_the_moment(device):
         case.v[int(case.table[b, at // 16]), :, at % 16] = kv[row].to(F64).cpu()
     held(got, *ref.attention(case, q0 * 2.0, causal=True))
     assert torch.equal(k[0].to(F64).cpu(), case.tokens("k", 0))
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_seeded_sweep(device, seed):
+    """Calls that draw everything at once: batch, lengths, heads, pages, types, masks, splits, rows around the sequences."""
+    r = np.random.default_rng(1000 + seed)
+    pick = lambda *x: x[int(r.integers(len(x)))]
+    d, page, dtype, coded = pick(64, 128, 256), pick(16, 32, 128, 1024), pick(BF16, F16), pick(False, True)
+    hkv, group = pick(1, 2, 3, 8), pick(1, 2, 4, 5, 8, 20)
+    batch, most = pick((1, 6000), (3, 2500), (20, 500), (90, 150))
+    new = pick(1, 1, 4, 40, 200)
+    if batch * new > 1500:
+        new = 4
+    context = [int(x) for x in np.exp(r.uniform(0, np.log(most), batch))]
+    fresh = [int(r.integers(0, new + 1)) if r.random() < 0.8 else min(1, new) for _ in range(batch)]
+    fresh[int(r.integers(batch))] = max(1, new)
+    causal = bool(r.random() < 0.8)
+    window = None if r.random() < 0.6 else (int(r.integers(0, 400)), int(r.integers(0, 100)) if not causal else 0)
+    opts = dict(causal=causal, window=window, scale=pick(None, 0.05, -0.03))
+    case = make(device, context, fresh, kv_heads=hkv, d=d, page=page, dtype=dtype, coded=coded, seed=seed,
+                rows_before=pick(0, 3), rows_after=pick(0, 33), wide=(pick(torch.int32, torch.int64), pick(torch.int32, torch.int64)),
+                columns=pick(None, 200 + 6400 // page))
+    q = normal((case.rows, hkv * group, d), dtype, seed, device)
+    splits = pick(None, None, None, 1, 2, 7)
+    out = torch.full_like(q, 3.0)
+    svod_amd.attention_paged(q, case.pages, Attn(splits=splits, **opts), out=out)
+    held(out, *ref.attention(case, q, **opts), (seed, svod_amd.chosen()))
+    s, e = case.starts[0], case.starts[-1]
+    assert bool((out[:s] == 3.0).all()) and bool((out[e:] == 3.0).all())
+    again = torch.full_like(q, 3.0)
+    svod_amd.attention_paged(q, case.pages, Attn(splits=splits, **opts), out=again)
+    assert torch.equal(bits(out), bits(again))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("fresh,h", [(5, 2), (40, 2), (200, 8)])
+def test_keys_that_a_row_does_not_see_may_hold_anything(device, fresh, h, bad):
+    """A new token's key that is no number: the rows in front of it, in its own tile and block, are what they were; a row behind sees it."""
+    case = make(device, [77], [fresh], kv_heads=1, d=64, page=16, seed=21)
+    q = normal((fresh, h, 64), BF16, 22, device)
+    want = svod_amd.attention_paged(q, case.pages, Attn(causal=True))
+    at = 77 + fresh // 2
+    case.pages.k[int(case.table[0, at // 16]), 0, at % 16, 3] = bad
+    got = svod_amd.attention_paged(q, case.pages, Attn(causal=True))
+    assert torch.equal(bits(got[:fresh // 2]), bits(want[:fresh // 2]))
+    assert torch.isfinite(want).all()
+    if bad != bad:
+        assert torch.isnan(got[fresh // 2:]).all()
