@@ -243,10 +243,13 @@ int svodk_order_rows(const svodk_tensor *keys, const svodk_tensor *order, void *
  * stand for more than the operands' type holds end at 240 * 2^e.  An infinity or a NaN is stored as NaN.
  *
  * `page` is a power of two from 16 to 1024, D 64, 128 or 256; others answer SVODK_GRAPH_SHAPE.  The table's
- * entries, lengths and starts are device data that no host check reads: they are held inside the pool, the
- * table (lens[b] <= columns * page) and the packed operands, so that a bad one gives a wrong result and never
- * an access out of bounds.  A sequence with fewer tokens than new rows has no position for the first of them:
- * they are not stored and see no key.  Rows in two sequences at once (starts that descend) may be left out.
+ * entries, lengths and starts are device data that no host check reads.  What reads the pages holds them
+ * inside the pool, the table (lens[b] <= columns * page) and the packed operands, so that a bad one gives a
+ * wrong result and never an access out of bounds.  svodk_write_pages stores a row at the position that the
+ * numbers name or not at all: rows of a position outside the table, and of an entry that is no page of the
+ * pool, are left out.  So a padded batch's rows may have entries of -1.  A sequence with fewer tokens than new
+ * rows has no position for the first of them: they are not stored and see no key.  Rows in two sequences at
+ * once (starts that descend) may be left out.
  */
 typedef struct svodk_pages {
   const svodk_tensor *k, *v;             /* [pages, kv_heads, page, D], one type */

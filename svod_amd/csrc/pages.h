@@ -5,9 +5,9 @@
 // [pages, kv_heads, page, D], so that a page holds a KV head's rows side by side: a stream of one head's keys runs in
 // pieces of page * D values, whatever the number of heads (rows of [page, kv_heads, D] would be pieces of D).
 //
-// All three integers are device data that no host check sees.  They are held inside what is there: a length inside the
-// table's columns, a row inside the packed operand, a page inside the pool.  A bad one gives a wrong result, never an access out
-// of bounds.
+// All three integers are device data that no host check sees.  What reads the cache holds them inside what is there: a length inside
+// the table's columns, a row inside the packed operand, a page inside the pool.  A bad one gives a wrong result, never an access out
+// of bounds.  What writes it may not: a place held inside is another token's.  A row goes to its own place or nowhere (Fresh).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -30,16 +30,26 @@ __device__ __forceinline__ int integer_at(const void *p, int64_t b, bool wide, i
   return n < 0 ? 0 : (n < (long long)most ? (int)n : most);
 }
 
-__device__ __forceinline__ Sequence sequence_at(const PagesArgs &p, int b) {
-  Sequence s;
-  s.len = integer_at(p.lens, b, p.lens_i64, p.columns << p.page_log2);
-  s.start = integer_at(p.starts, b, p.starts_i64, p.rows);
-  const int end = integer_at(p.starts, (int64_t)b + 1, p.starts_i64, p.rows);
-  s.fresh = end > s.start ? end - s.start : 0;
-  return s;
+// A sequence's new rows as they are written: those of [start, start + fresh) of the packed operands, row r at position shift + r,
+// which may be any.  Unlike a Sequence's, the position goes by the length and the end as they are given: the rows of a length past the
+// table, or of an end past the operands, would take the places of earlier tokens by the held ones.
+struct Fresh {
+  int start, fresh, shift;
+};
+__device__ __forceinline__ Fresh fresh_at(const PagesArgs &p, int b) {
+  auto given = [](const void *x, int64_t i, bool wide) { return wide ? ((const long long *)x)[i] : (long long)((const int *)x)[i]; };
+  Fresh f;
+  f.start = integer_at(p.starts, b, p.starts_i64, p.rows);
+  f.fresh = max(integer_at(p.starts, (int64_t)b + 1, p.starts_i64, p.rows) - f.start, 0);
+  // Rows and positions are below 2^30: a shift as far out leaves every row without a place, and the sum in 32 bits.
+  const long long far = 1ll << 30;
+  long long shift;
+  if (__builtin_sub_overflow(given(p.lens, b, p.lens_i64), given(p.starts, (int64_t)b + 1, p.starts_i64), &shift)) shift = far;
+  f.shift = (int)(shift < -far ? -far : shift > far ? far : shift);
+  return f;
 }
 
-// The page of a sequence's `column`-th run of `page` tokens.
+// The page of a sequence's `column`-th run of `page` tokens, to be read.
 __device__ __forceinline__ int page_at(const PagesArgs &p, int b, int column) {
   const int id = p.table[(int64_t)b * p.columns + min(column, p.columns - 1)];
   return min(max(id, 0), p.pages - 1);

@@ -130,8 +130,8 @@ __global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, u
   // The sequence and the position of each of the wave's rows: the sequences a lane each, 64 at a time.
   int b = -1, at = -1;
   for (int base = 0; base < p.batch; base += 64) {
-    Sequence s{};
-    if (base + lane < p.batch) s = sequence_at(p, base + lane);
+    Fresh s{};
+    if (base + lane < p.batch) s = fresh_at(p, base + lane);
     int found = 0;
 #pragma unroll
     for (int r = 0; r < kRows; r++) {
@@ -140,15 +140,17 @@ __global__ __launch_bounds__(kWaves * 64) void write_pages_kernel(PagesArgs p, u
       if (here != 0) {
         found++;
         const int one = __builtin_ctzll(here);
-        const int position = __builtin_amdgcn_readlane(s.base() - s.start, one) + (int)(row0 + r);
+        const int position = __builtin_amdgcn_readlane(s.shift, one) + (int)(row0 + r);
         if (lane / kLanes == r && b < 0) b = base + one, at = position;
       }
     }
     if (found == kRows) break;
   }
-  // A row of no sequence, or past what the length has room for, goes nowhere; its lanes go on, for their neighbours' sums.
-  const bool goes = there && b >= 0 && at >= 0;
-  const int page = goes ? page_at(p, b, at >> p.page_log2) : 0, in_page = at & ((1 << p.page_log2) - 1);
+  // A row of no sequence, of a position that the table has no column for, or of a page that the pool has not, goes nowhere; its
+  // lanes go on, for their neighbours' sums.
+  bool goes = there && b >= 0 && at >= 0 && at < p.columns << p.page_log2;
+  const int page = goes ? p.table[(int64_t)b * p.columns + (at >> p.page_log2)] : 0, in_page = at & ((1 << p.page_log2) - 1);
+  goes = goes && page >= 0 && page < p.pages;
 #pragma unroll
   for (int h = 0; h < HEADS; h++) {
     const bool writes = goes && head0 + h < p.kv_heads;

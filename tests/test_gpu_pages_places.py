@@ -1,0 +1,77 @@
+"""Rows of a step that have no place in a cache in pages, or none that is there: what write_pages stores."""
+import pytest
+import torch
+
+import svod_amd
+from svod_amd import Pages
+from pages_reference import make
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+KINDS = [(BF16, False), (F16, False), (BF16, True), (F16, True)]
+
+
+def bits(x):
+    return x.detach().cpu().contiguous().view(torch.uint8 if x.element_size() == 1 else torch.int16)
+
+
+def normal(shape, dtype, seed, device, by=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * by).to(dtype).to(device)
+
+
+# ---- write_pages: a row goes to its own position, or nowhere.
+def stored(table, lens, starts, rows, columns, page, count):
+    """(row, page, row of the page) of each packed row that has a place: the definition, on whole numbers of any size."""
+    for b in range(len(lens)):
+        for row in range(max(starts[b], 0), min(starts[b + 1], rows)):
+            at = lens[b] - (starts[b + 1] - row)
+            if 0 <= at < columns * page and 0 <= table[b][at // page] < count:
+                yield row, table[b][at // page], at % page
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+@pytest.mark.parametrize("name", ["pages that are none", "no page at all", "lengths past the table", "lengths far out", "ends past the rows"])
+@pytest.mark.parametrize("hkv,new", [(2, [5, 3, 40, 1]), (8, [900, 1, 800, 350])])
+def test_a_row_goes_to_its_place_or_nowhere(device, hkv, new, name, dtype, coded):
+    """Entries, lengths and starts out of range, beside sequences that are as they should be: nothing is written to a page or a
+    position that is not the row's own.  (The larger call takes four heads a wave.)"""
+    d, page = 128, 16
+    case = make(device, [37, 0, 70, 16], new, kv_heads=hkv, d=d, page=page, dtype=dtype, coded=coded, seed=hkv, fill=0.0, rows_after=3,
+                wide=(torch.int64, torch.int64))
+    lens, starts, table, rows, count = list(case.lens), list(case.starts), case.table.clone(), case.rows, case.k.shape[0]
+    columns = table.shape[1]
+    if name == "pages that are none":
+        table[0, -(-lens[0] // page) - 1] = -1
+        table[2, lens[2] // page // 2 + 2] = count
+        table[3, (lens[3] - 1) // page] = 0x7fffffff
+    elif name == "no page at all":
+        table[0] = -1
+        table[2] = -(1 << 31)
+        table[3] = count
+    elif name == "lengths past the table":
+        lens[0] = columns * page + 2
+        lens[2] = columns * page + new[2] - 1
+        lens[3] = columns * page + new[3]
+    elif name == "lengths far out":
+        lens[0], lens[2], lens[3] = (1 << 62), -(1 << 62), (1 << 32) + 5
+    else:
+        starts[4] = rows + 2  # two rows more than there are
+    # A place named twice would be a wrong test.
+    places = list(stored(table.tolist(), lens, starts, rows, columns, page, count))
+    assert len({(i, r) for _, i, r in places}) == len(places)
+    k, v = (normal((rows, hkv, d), dtype, s, "cpu", by=3.0) for s in (1, 2))
+    pages = Pages(case.pages.k, case.pages.v, table.to(device), torch.tensor(lens, device=device), torch.tensor(starts, device=device),
+                  case.pages.scales)
+    pools = [case.pages.k, case.pages.v, *(case.pages.scales or ())]
+    want = [bits(x).clone() for x in pools]
+    # The same rows by a call that has nothing out of range: one sequence of them all.
+    clean = make(device, [0], [rows], kv_heads=hkv, d=d, page=page, dtype=dtype, coded=coded, seed=0, fill=0.0)
+    svod_amd.write_pages(k.to(device), v.to(device), clean.pages)
+    own = [bits(x) for x in (clean.pages.k, clean.pages.v, *(clean.pages.scales or ()))]
+    for row, i, r in places:
+        for to, x in zip(want, own):
+            to[i, :, r] = x[int(clean.table[0, row // page]), :, row % page]
+    svod_amd.write_pages(k.to(device), v.to(device), pages)
+    for now, x in zip(pools, want):
+        assert torch.equal(bits(now), x)
