@@ -395,7 +395,8 @@ __device__ __forceinline__ int lowest_key(const PagedParams &p, const Work &w) {
 }
 
 // A lane's query row of a tile: query head row % group of the KV head's, of the tile's token row / group.  The keys [lo, hi] it
-// sees ascend with the row; rows past the last token stand in for it.
+// sees ascend with the row; rows past the last token stand in for it.  A token in front of its sequence's first (a length short of
+// its new rows) sees none, whatever the mask.
 struct Row {
   bool there;
   int64_t at;  // of (packed row, head), in heads
@@ -413,7 +414,7 @@ __device__ __forceinline__ Row row_of_tile(const Deal &deal, const PagedParams &
   if (p.causal) hi = min(hi, pos);
   if (p.win_left >= 0) lo = max(lo, pos - p.win_left), hi = min(hi, pos + p.win_right);
   r.lo = lo;
-  r.hi = max(hi, -1);
+  r.hi = pos < 0 ? -1 : max(hi, -1);
   return r;
 }
 

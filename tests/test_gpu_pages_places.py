@@ -1,9 +1,10 @@
-"""Rows of a step that have no place in a cache in pages, or none that is there: what write_pages stores."""
+"""Rows of a step that have no place in a cache in pages, or none that is there: what write_pages stores and attention_paged sees."""
 import pytest
 import torch
 
 import svod_amd
-from svod_amd import Pages
+from svod_amd import Attn, Pages
+import pages_reference as ref
 from pages_reference import make
 
 pytestmark = pytest.mark.gpu
@@ -18,6 +19,13 @@ def bits(x):
 
 def normal(shape, dtype, seed, device, by=1.0):
     return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * by).to(dtype).to(device)
+
+
+def held(got, want, allowed, what=""):
+    got, rows = got.double().cpu(), ~torch.isnan(want)
+    assert torch.isfinite(got[rows]).all(), what
+    off = (got - want).abs()[rows]
+    assert not (off > allowed[rows]).any(), (what, float((off - allowed[rows]).max()))
 
 
 # ---- write_pages: a row goes to its own position, or nowhere.
@@ -75,3 +83,27 @@ def test_a_row_goes_to_its_place_or_nowhere(device, hkv, new, name, dtype, coded
     svod_amd.write_pages(k.to(device), v.to(device), pages)
     for now, x in zip(pools, want):
         assert torch.equal(bits(now), x)
+
+
+# ---- attention_paged: a row in front of its sequence's first token sees no key.
+MASKS = {"none": {}, "causal": dict(causal=True), "both sides": dict(window=(33, 65)), "right": dict(window=(0, 500)),
+         "causal window": dict(causal=True, window=(40, 0)), "a negative scale": dict(scale=-0.2)}
+
+
+@pytest.mark.parametrize("dtype,coded", KINDS)
+@pytest.mark.parametrize("name", MASKS)
+@pytest.mark.parametrize("lens,new,h,splits", [([4, 0, 70], [6, 9, 3], 4, None),            # tiles of 16 rows
+                                               ([2, 700, 1], [17, 20, 5], 4, 3),             # split ones, of 32
+                                               ([100, 0, 90], [300, 40, 2], 4, None),       # of 128: a tile without a position, one across
+                                               ([900, 64], [1100, 200], 4, 4)])             # and split
+def test_a_row_without_a_position_sees_no_key(device, lens, new, h, splits, name, dtype, coded):
+    opts = MASKS[name]
+    case = make(device, [0] * len(new), new, kv_heads=2, d=64, lens=lens, dtype=dtype, coded=coded, seed=len(name))
+    q = normal((case.rows, h, 64), dtype, 13, device)
+    out = svod_amd.attention_paged(q, case.pages, Attn(splits=splits, **opts))
+    want, allowed = ref.attention(case, q, **opts)
+    for b, (n, t) in enumerate(zip(lens, new)):
+        none = slice(case.starts[b], case.starts[b] + max(0, t - n))
+        assert bool((out[none] == 0).all()), b
+        want[none] = 0.0  # whatever the mask
+    held(out, want, allowed, name)
