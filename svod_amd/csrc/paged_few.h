@@ -362,8 +362,7 @@ __device__ __forceinline__ void item(uint8_t *smem, const Deal &deal, const Page
 
   if (counts && (found >> kPagedCountBits != p.tag || (found & kPagedEnded) == kPagedEnded))
     __hip_atomic_compare_exchange_strong(word, &found, p.tag << kPagedCountBits, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // ---- the waves' states as one: maxima in the exponent's units.
-  if (L::kState > L::kTile) __syncthreads();  // a state reaches into the next wave's tile
+  // ---- the waves' states as one: maxima in the exponent's units.  A wave's state lies where its tile of V did.
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const float sum = over_quarters(l[t], [](float a, float b) { return a + b; });
