@@ -573,7 +573,10 @@ int64_t paged_slots(const PagedArgs &a) {
   // tiles, 34.9 us with it and 32.1 without, nothing split in either).  And blocks of all tiles are counted in 31 bits.
   const int64_t least = few ? (dense(a) ? 32 : 9) : dense(a) ? 64 : rounds(a) > 1 ? 24 : 5;
   if (blocks < least || tiles / a.pages.kv_heads * blocks > 0x3fffffff) return 0;
-  return few && dense(a) ? 2 * (places(a) + a.pages.kv_heads) : paged_workgroups(a);
+  // Two a workgroup of the places, none for one that the launch has not: of a tile that such a one shared (where sums over starts that
+  // descend have wrapped) the others would count themselves in, and leave its word between two counts for the next replay.
+  const int64_t round = a.pages.kv_heads;
+  return few && dense(a) ? 2 * ((places(a) + round) / round * round) : paged_workgroups(a);
 }
 
 // The workgroups of a launch: for every tile there may be, and for the chip's places where tiles may be split; for half of those more
