@@ -107,3 +107,52 @@ def test_a_row_without_a_position_sees_no_key(device, lens, new, h, splits, name
         assert bool((out[none] == 0).all()), b
         want[none] = 0.0  # whatever the mask
     held(out, want, allowed, name)
+
+
+# ---- attention_paged: numbers out of range, in every form of a launch.
+FORMS = {  # contexts, new tokens, query heads, kv heads, D, splits
+    "few rows, whole and in parts": ([3000, 40, 500, 9], [1, 2, 1, 3], 4, 2, 64, None),
+    "few rows, named splits": ([3000, 40, 500, 9], [1, 2, 1, 3], 4, 2, 128, 5),
+    "shares": ([100 + 7 * (i % 40) for i in range(146)] + [9000, 6000, 4000, 7000], [1] * 150, 4, 4, 64, None),
+    "32 rows": ([2500, 700, 64, 3], [8, 5, 9, 2], 8, 2, 128, None),
+    "chunks": ([300, 0, 77, 500], [200, 150, 1, 30], 4, 2, 64, 1),
+    "chunks in parts": ([3000, 700, 64, 2000], [150, 30, 200, 1], 4, 2, 128, None),
+    "chunks, named splits": ([3000, 700, 64, 2000], [150, 30, 200, 1], 4, 2, 64, 3),
+}
+
+
+@pytest.mark.parametrize("coded", [False, True])
+@pytest.mark.parametrize("bad", ["a length past the table", "a length far past it", "a negative length", "pages that are none", "an end past the rows"])
+@pytest.mark.parametrize("name", FORMS)
+def test_numbers_out_of_range_stay_with_their_sequence(device, name, bad, coded):
+    """One sequence's length, entries or end are wrong: its own rows hold something, those of the others what they should, and nothing beside
+    the rows and in the pools is touched."""
+    context, new, h, hkv, d, splits = FORMS[name]
+    case = make(device, context, new, kv_heads=hkv, d=d, coded=coded, seed=len(name), fill=0.0, rows_after=2, wide=(torch.int64, torch.int64))
+    q = normal((case.rows, h, d), BF16, 5, device)
+    want, allowed = ref.attention(case, q, causal=True)
+    one = len(new) - 1 if bad == "an end past the rows" else 1
+    lens, starts, table = case.pages.lens.clone(), case.pages.starts.clone(), case.pages.table.clone()
+    limit = table.shape[1] * 16
+    if bad == "a length past the table":
+        lens[one] = limit + 5
+    elif bad == "a length far past it":
+        lens[one] = 1 << 60
+    elif bad == "a negative length":
+        lens[one] = -(1 << 33) + 70
+    elif bad == "pages that are none":
+        table[one, ::2], table[one, 1::2] = -7, 0x7fffffff
+    else:
+        starts[one + 1] = case.rows + (1 << 35)
+    pages = Pages(case.pages.k, case.pages.v, table, lens, starts, case.pages.scales)
+    pools = [case.pages.k, case.pages.v, *(case.pages.scales or ())]
+    before = [bits(x).clone() for x in pools]
+    guard = torch.full((case.rows + 64, h, d), 5.0, dtype=BF16, device=device)
+    out = svod_amd.attention_paged(q, pages, Attn(causal=True, splits=splits), out=guard[32:32 + case.rows])
+    assert bool((guard[:32] == 5.0).all()) and bool((guard[32 + case.rows:] == 5.0).all()) and torch.isfinite(out).all()
+    want[case.starts[one]:case.starts[one + 1]] = float("nan")  # its own rows
+    held(out, want, allowed, name)
+    for x, was in zip(pools, before):
+        assert torch.equal(bits(x), was)
+    # Good numbers in the same places: the call is what it was.
+    held(svod_amd.attention_paged(q, case.pages, Attn(causal=True, splits=splits)), *ref.attention(case, q, causal=True))
