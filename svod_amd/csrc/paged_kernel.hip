@@ -569,9 +569,20 @@ int64_t paged_slots(const PagedArgs &a) {
   const bool few = paged_tile_rows(a) != 128;
   // A state for each of many tiles of 128 rows would be gigabytes, where none is more than a small part of the launch.
   if (!few && tiles > 4 * places(a)) return 0;
-  // Too short to be worth a merge, whatever the lengths: for tiles of 128 rows it is a launch (two chunks of 1001 in a window of 1024, 256
-  // tiles, 34.9 us with it and 32.1 without, nothing split in either).  And blocks of all tiles are counted in 31 bits.
-  const int64_t least = few ? (dense(a) ? 32 : 9) : dense(a) ? 64 : rounds(a) > 1 ? 24 : 5;
+  // Too short to be worth a merge, whatever the lengths.  (us whole, and as the device deals it out from the bound on; 16 query heads over 8
+  // of 128 in 16 bits, a key block 64 keys.)
+  //   few rows, 9: one sequence of 8 blocks 11.3, in four splits 10.3, 16 sequences 12.8 and 14.4; one of 9 13.4 and 14.1, of 10 13.4 and 11.8, 16
+  //   of 10 15.2 and 15.8, of 16 19.2 and 19.6.
+  //   few rows, dense, 32: no shares win below (40 sequences of 110 to 1100 keys 28.6 and 35.0), and from there on they may (300 to 3000 75.1 and
+  //   65.1); a call that does not take any pays 1.5 for having the choice (64 of 204 to 2048 62.6 and 64.1).
+  // Of 128 rows the merge is a launch, paid for split or not:
+  //   8: a chunk of 128 in 7 blocks 14.6, in four splits 15.0; in 8 15.4 and 15.6 (codes 18.6 and 16.5; heads of 256 22.4 and 19.6; of
+  //   64 11.2 and 12.3), in 10 17.8 and 16.2.
+  //   two rounds of places, 24: two chunks of 512 in 22 blocks 33.3, in two to four splits 33.3; in 24 35.7 and 35.5, in 32 45.2 and 39.1.
+  //   dense, 64: two chunks of 1001 in a window of 1024, 256 tiles, 32.1, and 34.9 with the merge's launch; what is given up is a long
+  //   sequence among short ones (20 chunks of 256, one of them in 63 blocks and the others in 300 keys, 96.4; in 64 97.2 and 63.8).
+  // And blocks of all tiles are counted in 31 bits.
+  const int64_t least = few ? (dense(a) ? 32 : 9) : dense(a) ? 64 : rounds(a) > 1 ? 24 : 8;
   if (blocks < least || tiles / a.pages.kv_heads * blocks > 0x3fffffff) return 0;
   // Two a workgroup of the places, none for one that the launch has not: of a tile that such a one shared (where sums over starts that
   // descend have wrapped) the others would count themselves in, and leave its word between two counts for the next replay.

@@ -22,3 +22,15 @@ def test_shares_have_states_for_the_workgroups_that_are_launched(kv_heads, coded
     workgroups = max(batch * kv_heads, on_places)
     state = 16 * (d + 2) * 4
     assert svod_amd.attention_paged_workspace(q, pages, Attn(causal=True)) == 2 * on_places * state + workgroups * 128
+
+
+def test_a_chunk_over_few_keys_is_not_split():
+    """Below eight key blocks a tile of 128 rows stays whole whatever the lengths, so that no merge is launched."""
+    def bytes_of(keys, d=128):
+        pool = lambda: torch.zeros(4, 8, 64, d, dtype=torch.bfloat16)
+        pages = Pages(pool(), pool(), torch.zeros(1, keys // 64, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
+                      torch.zeros(2, dtype=torch.int32))
+        return svod_amd.attention_paged_workspace(torch.zeros(128, 16, d, dtype=torch.bfloat16), pages, Attn(causal=True))
+
+    for d in (64, 128, 256):
+        assert [bytes_of(64 * n, d) > 0 for n in (1, 4, 5, 7, 8, 9)] == [False] * 4 + [True] * 2
