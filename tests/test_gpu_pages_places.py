@@ -156,3 +156,22 @@ def test_numbers_out_of_range_stay_with_their_sequence(device, name, bad, coded)
         assert torch.equal(bits(x), was)
     # Good numbers in the same places: the call is what it was.
     held(svod_amd.attention_paged(q, case.pages, Attn(causal=True, splits=splits)), *ref.attention(case, q, causal=True))
+
+
+def test_codes_past_the_other_types_range_are_infinite(device):
+    """A pool written from bf16 and read in f16: a row is rounded to it, codes from 65520 on (the middle between its largest value and the
+    next) to an infinity, the others in place."""
+    codes = torch.arange(0x80, dtype=torch.uint8)[:0x7f].repeat(2, 1)  # both halves: every finite code of one sign, and its negative
+    codes[1] |= 0x80
+    codes = torch.nn.functional.pad(codes, (0, 1)).expand(1, 1, 8, 2, 128).reshape(1, 1, 16, 128).contiguous()
+    e = torch.arange(4, 12).repeat_interleave(2)
+    scales = (e + 127).to(torch.uint8).view(1, 1, 16)
+    pool, scale = codes.to(device).view(ref.E4M3), scales.to(device).view(ref.E8M0)
+    pages = Pages(pool, pool, torch.zeros(1, 1, dtype=torch.int32, device=device), torch.tensor([16], dtype=torch.int32, device=device),
+                  scales=(scale, scale))
+    stood = codes[0, 0].view(ref.E4M3).double() * torch.pow(2.0, e.double())[:, None]
+    want = torch.where(stood.abs() >= 65520, stood.sign() * float("inf"), stood)  # what fits is exact: four significant bits
+    for x in svod_amd.read_pages(pages, 16, F16):
+        assert torch.equal(x[0, :, 0].double().cpu(), want)
+    for x in svod_amd.read_pages(pages, 16, BF16):
+        assert torch.equal(x[0, :, 0].double().cpu(), stood)
