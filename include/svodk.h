@@ -241,6 +241,8 @@ int svodk_order_rows(const svodk_tensor *keys, const svodk_tensor *order, void *
  * stands for code * scale.  Row x is stored with the scale 2^e, e the least whole number from -117 on with
  * max|x| <= 448 * 2^e over its finite values, and codes x / 2^e rounded to the nearest even; codes that would
  * stand for more than the operands' type holds end at 240 * 2^e.  An infinity or a NaN is stored as NaN.
+ * A pool of codes may be read in the other 16-bit type: a row is rounded to it then, so that in f16 what was
+ * written from bf16 and lies past 65504 is infinite.
  *
  * `page` is a power of two from 16 to 1024, D 64, 128 or 256; others answer SVODK_GRAPH_SHAPE.  The table's
  * entries, lengths and starts are device data that no host check reads.  What reads the pages holds them
@@ -278,7 +280,8 @@ int svodk_read_pages(const svodk_pages *pages, const svodk_tensor *k, const svod
  * op of svodk_attention with each query at its token's position p.  causal: keys 0 .. p, the token's own among
  * them (svodk_write_pages comes first); a window: keys p - left .. p + right; neither: all lens[b].  A query that
  * sees no key comes out as zeros.  Of the options causal, window, scale, splits and workspace count; any other
- * that is set answers SVODK_GRAPH_CONFIG, as does a named count of splits without the workspace it needs.
+ * that is set answers SVODK_GRAPH_CONFIG, as does a named count of splits without the workspace it needs, or
+ * one that would need more than 2 GiB.
  * More than 128 query heads a KV head answer SVODK_GRAPH_SHAPE.
  *
  * `splits` = 0 splits the keys of long sequences where the workspace svodk_attention_paged_workspace asks for

@@ -108,9 +108,12 @@ __device__ __forceinline__ int sum_to(int x) {
 
 constexpr float kStart = 5.0f, kMerge = 5.0f;  // us: from a part's place to its first block, and the merge
 // A share of all blocks: how much of the time of uneven tiles its blocks take, its own start and its two merges in us, and a tile's start in it.
-// (With PagedParams' tail and even from 98 calls of 30 to 128 sequences of 500 to 8000 keys, each whole and in shares: what is chosen is
-// 0.4 % over the better on average, 7 % at most.  Shares win where lengths differ and are long: 40 sequences of 1600 to 8000 keys, 8
-// KV heads of 128, whole 197 us, 148 in shares; of 110 to 1100 keys 28.6 and 35.)
+// (Fitted, with PagedParams' tail and even, on 98 calls of a token each of 30 to 128 sequences of 500 to 8000 keys, whole and in shares.  Over 48 that
+// it was not fitted on, of 40 to 200 sequences of 100 to 9000 keys, head sizes 64, 128 and 256, both kinds of pools, tiles of 16 and 32 rows
+// and a window, what is chosen is 0.7 % over the better of whole and chosen on average and 7.6 % at most, 200 sequences of 500 to 2500 keys, 8
+// KV heads of 128 in codes, 143 us where whole is 133; whole throughout would be 11 % over.  Shares win where lengths differ and are long: 40
+// sequences of 1600 to 8000 keys whole 197 us, 148 in shares; of 110 to 1100 keys 28.6 and 35.  It knows nothing of a chunk, whose many
+// tiles read the same keys: one of 2048 beside 255 tokens over 600 keys, 16 query heads over 8 of 128, takes 480 in shares and 296 whole.)
 constexpr float kShareOf = 0.8f, kShare = 14.0f, kShareTile = 9.0f;
 // What a lane's sequence asks for: tiles of query rows, and the key blocks of one of its tiles at most.
 struct Demand {

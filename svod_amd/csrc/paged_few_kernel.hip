@@ -1,5 +1,7 @@
-// Attention over a key/value cache in pages where every sequence has few query rows a KV head: tiles of 16 or 32 rows
-// (paged_few.h), on places that a compute unit has for one to three workgroups.
+// Attention over a key/value cache in pages where sequences have few query rows a KV head on average, 16 or 32: tiles of as many rows
+// (paged_few.h), on places that a compute unit has for one to three workgroups.  The host knows the mean alone, so a long chunk among
+// many single tokens comes here too, as many tiles: it is right so, and slow (one of 449 beside 63 tokens over 4096 keys, 32 query heads
+// over 8 of 128: 289 us here, 209 in tiles of 128 rows).
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"

@@ -390,7 +390,8 @@ def write_pages(k: torch.Tensor, v: torch.Tensor, pages: Pages) -> None:
 def read_pages(pages: Pages, tokens: int, dtype: Optional[torch.dtype] = None,
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Positions ``0 .. tokens - 1`` of every sequence as ``(k, v)`` ``[B, tokens, kv_heads, D]``, zeros past its end: the
-    layout of ``attention``'s keys.  ``dtype``: of rows that are held in 8 bits, bfloat16 unless named."""
+    layout of ``attention``'s keys.  ``dtype``: of rows that are held in 8 bits, bfloat16 unless named (in float16 what lies past 65504,
+    as rows written from bfloat16 may, is infinite)."""
     return (_native or _calls()).read_pages(pages, tokens, dtype, out, _fresh if POISON else None)
 
 
@@ -399,7 +400,9 @@ def attention_paged(q: torch.Tensor, pages: Pages, opts: Optional[Attn] = None, 
     """``attention`` of the new tokens' queries ``[N, H, D]``, each at its token's position, over the pages of its sequence;
     returns ``[N, H, D]``.  ``opts``: ``causal`` (a token sees itself: ``write_pages`` comes first), ``window``, ``scale`` and
     ``splits``.  With ``splits`` ``None`` the device splits the keys of long sequences, by all the lengths: a row's last bits may
-    depend on them.  Rows of no sequence stay as they are in ``out``."""
+    depend on them.  Rows of no sequence (in front of ``starts[0]``, from ``starts[B]`` on) are not written: in ``out`` they stay as they
+    are, and without one they hold what the memory held, NaN perhaps, as the batches past a ``batch_live`` do.  A padded step whose next
+    ops look at all rows lends an ``out`` that was cleared once."""
     return (_native or _calls()).attention_paged(q, pages, opts, out, workspace, _fresh if POISON else None)
 
 
