@@ -383,7 +383,8 @@ class Pages:
 
 def write_pages(k: torch.Tensor, v: torch.Tensor, pages: Pages) -> None:
     """The new tokens' keys and values ``[N, kv_heads, D]`` into their pages, quantised where those hold 8 bits.  Rows of no
-    sequence are left out, and so are rows whose position the table has no column for, or whose entry is no page of the pool.  Enqueued on the current stream of ``k``'s device, as every op."""
+    sequence are left out, and so are rows whose position the table has no column for or whose entry is no page of the pool.
+    Enqueued on the current stream of ``k``'s device, as every op."""
     (_native or _calls()).write_pages(k, v, pages)
 
 
