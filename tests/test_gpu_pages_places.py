@@ -41,12 +41,13 @@ def stored(table, lens, starts, rows, columns, page, count):
 @pytest.mark.parametrize("dtype,coded", KINDS)
 @pytest.mark.parametrize("name", ["pages that are none", "no page at all", "lengths past the table", "lengths far out", "ends past the rows"])
 @pytest.mark.parametrize("hkv,new", [(2, [5, 3, 40, 1]), (8, [900, 1, 800, 350])])
-def test_a_row_goes_to_its_place_or_nowhere(device, hkv, new, name, dtype, coded):
+@pytest.mark.parametrize("wide", [torch.int64, torch.int32])
+def test_a_row_goes_to_its_place_or_nowhere(device, wide, hkv, new, name, dtype, coded):
     """Entries, lengths and starts out of range, beside sequences that are as they should be: nothing is written to a page or a
     position that is not the row's own.  (The larger call takes four heads a wave.)"""
     d, page = 128, 16
     case = make(device, [37, 0, 70, 16], new, kv_heads=hkv, d=d, page=page, dtype=dtype, coded=coded, seed=hkv, fill=0.0, rows_after=3,
-                wide=(torch.int64, torch.int64))
+                wide=(wide, wide))
     lens, starts, table, rows, count = list(case.lens), list(case.starts), case.table.clone(), case.rows, case.k.shape[0]
     columns = table.shape[1]
     if name == "pages that are none":
@@ -62,15 +63,16 @@ def test_a_row_goes_to_its_place_or_nowhere(device, hkv, new, name, dtype, coded
         lens[2] = columns * page + new[2] - 1
         lens[3] = columns * page + new[3]
     elif name == "lengths far out":
-        lens[0], lens[2], lens[3] = (1 << 62), -(1 << 62), (1 << 32) + 5
+        far = torch.iinfo(wide)
+        lens[0], lens[2], lens[3] = far.max, far.min, (1 << 32) + 5 if wide == torch.int64 else far.max // 2
     else:
         starts[4] = rows + 2  # two rows more than there are
     # A place named twice would be a wrong test.
     places = list(stored(table.tolist(), lens, starts, rows, columns, page, count))
     assert len({(i, r) for _, i, r in places}) == len(places)
     k, v = (normal((rows, hkv, d), dtype, s, "cpu", by=3.0) for s in (1, 2))
-    pages = Pages(case.pages.k, case.pages.v, table.to(device), torch.tensor(lens, device=device), torch.tensor(starts, device=device),
-                  case.pages.scales)
+    pages = Pages(case.pages.k, case.pages.v, table.to(device), torch.tensor(lens, dtype=wide, device=device),
+                  torch.tensor(starts, dtype=wide, device=device), case.pages.scales)
     pools = [case.pages.k, case.pages.v, *(case.pages.scales or ())]
     want = [bits(x).clone() for x in pools]
     # The same rows by a call that has nothing out of range: one sequence of them all.
